@@ -205,6 +205,42 @@ int trx_gemv_packed_parts_f32(const uint8_t* packed, int kind, int M, int K, con
                               const float* resid, void* workspace, const trx_partial_sums* parts,
                               trx_stream_t s);
 
+/* Window attention over a KV ring ----------------------------------------------------------------
+ * Attention of the next n positions pos .. pos + n - 1 with a sliding window and a few first
+ * positions that stay visible (sinks), over a ring of K and V rows laid out as the decoder's: fp16
+ * [n_kv_head][slots][head_dim], position p in slot p where p < pin, else in slot
+ * pin + (p - pin) % (slots - pin) (firmware/hybrid.c:156-181 kv_slot). The query at position t sees
+ * u <= t with u < sinks or u > t - window:
+ *   out = sum e^(scale q.k_u) v_u / sum e^(scale q.k_u), times sigmoid(gate) with gate != NULL
+ * (model/fastref.py:31-43 attention_fp32, :216-241). n = 1 is the decode form.
+ * kind: TRX_KIND_F32 or TRX_KIND_F16, the type of q, gate and out. Row r of q has head h at
+ * r * q_stride + h * head_dim, of out at r * out_stride + h * head_dim, of gate at r * gate_stride +
+ * h * gate_head_stride; row r of k and v (fp16, post-RoPE, position pos + r) has kv head g at
+ * r * kv_stride + g * head_dim. Strides are in elements: q_stride a multiple of 16 bytes, kv_stride of
+ * 8, the others of 4; every pointer is 16-byte aligned.
+ * head_dim 64, 128 or 256; 0 <= sinks <= pin < slots, 1 <= window <= slots - pin, scale > 0, n >= 0
+ * (0: nothing is done).
+ * The ring holds the positions below pos that a query sees; slots that no visible position takes may
+ * hold anything. Afterwards the new rows stand in their slots (of rows that share a slot, the last);
+ * no other slot is written. An infinity or NaN in a key or value that a query does not see does not
+ * reach its output. out, workspace and the ring overlap no other argument.
+ * pos_dev != NULL: the first position is read from the device when the work runs (for captured
+ * graphs) and `pos` is ignored; a position there that is negative or leaves int32 within n leaves out
+ * and the ring as they are.
+ * workspace: trx_attn_window_geometry's bytes (may be 0: NULL then), no zeroing needed; calls that
+ * share it must not overlap. */
+typedef struct trx_attn_window_shape {
+  int kind;
+  int n_head, n_kv_head, head_dim;
+  int slots, pin, window, sinks;
+  int q_stride, kv_stride, out_stride, gate_stride, gate_head_stride;
+  float scale;
+} trx_attn_window_shape;
+int trx_attn_window_geometry(const trx_attn_window_shape* shape, int n, size_t* workspace_bytes);
+int trx_attn_window(const trx_attn_window_shape* shape, int n, int pos, const int32_t* pos_dev, const void* q,
+                    const uint16_t* k, const uint16_t* v, uint16_t* kcache, uint16_t* vcache,
+                    const void* gate, void* out, void* workspace, trx_stream_t s);
+
 /* Decoder ----------------------------------------------------------------------------------------
  * A batch-1 greedy decoder over a BONS model held on the GPU: the GPU counterpart of
  * model/golden.py:FloatModel (reset/forward/generate, golden.py:304-320,436-470) with the

@@ -48,6 +48,13 @@ class PartialSums(ctypes.Structure):
                 ("act", ctypes.c_void_p)]
 
 
+class AttnWindowShape(ctypes.Structure):
+    """trx_attn_window_shape (include/trixium.h): heads, ring and strides of the window attention."""
+    _fields_ = [(n, ctypes.c_int) for n in ("kind", "n_head", "n_kv_head", "head_dim", "slots", "pin", "window",
+                                            "sinks", "q_stride", "kv_stride", "out_stride", "gate_stride",
+                                            "gate_head_stride")] + [("scale", ctypes.c_float)]
+
+
 SIGNATURES = {
     "trx_last_error": [],
     "trx_version": [],
@@ -83,6 +90,8 @@ SIGNATURES = {
     "trx_gemv_packed_batched_f32": [_vp, _sz, _i, _i, _i, _i, _i, _vp, _i, _vp, _i, _vp, _vp],
     "trx_gemv_packed_parts_f32": [_vp, _i, _i, _i, _vp, _vp, _f, _vp, _i, _vp, _vp, _vp, _vp],
     "trx_gemv_set_variant": [_i],
+    "trx_attn_window_geometry": [ctypes.POINTER(AttnWindowShape), _i, ctypes.POINTER(_sz)],
+    "trx_attn_window": [ctypes.POINTER(AttnWindowShape), _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
     "trx_model_create": [_mcp, _fp, ctypes.POINTER(_vp)],
     "trx_model_destroy": [_vp],
     "trx_model_set_tensor": [_vp, _i, _i, _vp, _sz],
