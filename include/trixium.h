@@ -241,6 +241,36 @@ int trx_attn_window(const trx_attn_window_shape* shape, int n, int pos, const in
                     const uint16_t* k, const uint16_t* v, uint16_t* kcache, uint16_t* vcache,
                     const void* gate, void* out, void* workspace, trx_stream_t s);
 
+/* Sampling from the whole vocabulary --------------------------------------------------------------
+ * One token per row of logits by temperature, top-k, top-p and min-p from a given uniform number (the
+ * firmware's sampler, firmware/infer.c:385-488, draws among 32 candidates; trx_model_set_sampling).
+ * Tokens stand in the order of their logits, largest first, equal ones by index. The first top_k
+ * stay; of those the smallest prefix that holds at least top_p of their mass e^((logit - max) / T);
+ * of those the ones whose mass is at least min_p of the largest. tokens[r] is the first index, in
+ * index order, at which the mass that stayed exceeds u[r] times its total; logp[r] (may be NULL) the
+ * log of its share of that total.
+ * Masses are integers of 62 - ceil(log2 vocab) fractional bits (at most 51), evaluated in 64 bits, so
+ * a row's token depends on nothing but the row, its settings and u; a token below half a unit of the
+ * largest one's last bit cannot be drawn.
+ * Out of range: a temperature that is not above 0 (or NaN) takes the largest logit (logp 0); top_k
+ * outside [1, vocab), top_p outside (0, 1) and min_p outside [0, 1] are off; u is taken to the
+ * nearest value in [0, 1). A NaN logit counts as -inf; a row without a logit above -inf gives
+ * token -1 and logp NaN; tokens of +inf share the mass.
+ * kind: TRX_KIND_F32 or TRX_KIND_F16; row r at logits + r * ld (elements, ld >= vocab; any alignment
+ * of the type's own). rows: device array of n settings (per_row), or one for every row. vocab <= 2^24,
+ * n <= 2^20 (0: nothing is done). workspace: trx_sample_rows_geometry's bytes, 16-byte aligned, no
+ * zeroing needed; calls that share it must not overlap. */
+typedef struct trx_sampling {
+  float temperature;
+  int32_t top_k;
+  float top_p;
+  float min_p;
+} trx_sampling;
+int trx_sample_rows_geometry(int vocab, int n, size_t* workspace_bytes);
+int trx_sample_rows(const void* logits, int kind, int n, int vocab, int64_t ld, const trx_sampling* rows,
+                    int per_row, const float* u, int32_t* tokens, float* logp, void* workspace,
+                    trx_stream_t s);
+
 /* Decoder ----------------------------------------------------------------------------------------
  * A batch-1 greedy decoder over a BONS model held on the GPU: the GPU counterpart of
  * model/golden.py:FloatModel (reset/forward/generate, golden.py:304-320,436-470) with the

@@ -92,6 +92,8 @@ SIGNATURES = {
     "trx_gemv_set_variant": [_i],
     "trx_attn_window_geometry": [ctypes.POINTER(AttnWindowShape), _i, ctypes.POINTER(_sz)],
     "trx_attn_window": [ctypes.POINTER(AttnWindowShape), _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "trx_sample_rows_geometry": [_i, _i, ctypes.POINTER(_sz)],
+    "trx_sample_rows": [_vp, _i, _i, _i, ctypes.c_int64, _vp, _i, _vp, _vp, _vp, _vp, _vp],
     "trx_model_create": [_mcp, _fp, ctypes.POINTER(_vp)],
     "trx_model_destroy": [_vp],
     "trx_model_set_tensor": [_vp, _i, _i, _vp, _sz],
