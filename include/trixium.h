@@ -378,6 +378,14 @@ int trx_model_create(const trx_model_config* cfg, const float* rope_freq, trx_mo
    argmax (no extra launch). */
 int trx_model_set_sampling(trx_model* m, float temperature, float top_p, float repetition, uint32_t seed,
                            int n_channels);
+/* Sampling from the whole vocabulary instead (trx_sample_rows; the firmware's candidates are 32 at most):
+   the same repetition penalty, on every token of the last 64, then temperature, top_k, top_p and min_p
+   with u the next number of the firmware's xorshift32 stream (seed 0 keeps it), drawn where the
+   temperature is above 0. Settings out of range as in trx_sample_rows, a repetition below 1 is 1.
+   temperature 0 with repetition 1 is the greedy argmax. The last call of the two sets the sampler.
+   The logits that TRX_READ_LOGITS gives are without the penalty. */
+int trx_model_set_vocab_sampling(trx_model* m, float temperature, int top_k, float top_p, float min_p,
+                                 float repetition, uint32_t seed);
 int trx_model_destroy(trx_model* m);
 /* Upload one tensor (synchronous). Ternary and Q8: BONS row packets of the model's kind; F32:
  * float32 values; F16 head: fp16 values; TOK_EMB16: int16 [vocab, n_embd]; TOK_EMB16_EXP: int32
@@ -413,8 +421,7 @@ int trx_model_checkpoint(trx_model* m, int op);
  * default (on for a model with DeltaNet layers, as the firmware's hybrid; off otherwise, which
  * stops at max_ctx as the firmware's Qwen3 loop does). Both take effect at the next reset, and the
  * pin lasts one reset (then 4 again); the ring stays off where max_ctx <= 2 pin. A model whose
- * image carries a RoPE table (no rows past max_ctx) cannot turn it on: TRX_E_INVALID. Positions
- * past the window run one position per forward (trx_model_prefill steps them). */
+ * image carries a RoPE table (no rows past max_ctx) cannot turn it on: TRX_E_INVALID. */
 int trx_model_set_kv_ring(trx_model* m, int enable, int pin);
 /* Feed tokens at the next n positions (after the forwards already enqueued); logits are computed
  * from absolute position head_from on (-1: the last fed token). */
@@ -427,7 +434,9 @@ int trx_model_step(trx_model* m, int n_steps, int use_graph);
  * a GEMM over the chunk on the matrix cores, attention is causal over the cache, the DeltaNet
  * recurrence runs over the chunk's positions in order. The positions must precede head_from (no
  * logits); afterwards the KV cache, the DeltaNet state and the position are those of n
- * one-position forwards, and the next trx_model_step continues from there. */
+ * one-position forwards, and the next trx_model_step continues from there. Positions past max_ctx
+ * (the KV ring) run in chunks of their own over the ring (trx_attn_window's attention), fewer than
+ * four of them one forward each. */
 int trx_model_prefill(trx_model* m, int n, int chunk);
 /* Resolve the argmax of the last forward into the output buffer. */
 int trx_model_finalize(trx_model* m);

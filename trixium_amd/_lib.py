@@ -98,6 +98,7 @@ SIGNATURES = {
     "trx_model_destroy": [_vp],
     "trx_model_set_tensor": [_vp, _i, _i, _vp, _sz],
     "trx_model_set_sampling": [_vp, ctypes.c_float, ctypes.c_float, ctypes.c_float, ctypes.c_uint32, _i],
+    "trx_model_set_vocab_sampling": [_vp, _f, _i, _f, _f, _f, ctypes.c_uint32],
     "trx_model_synthesize": [_vp, ctypes.c_uint32, _fp],
     "trx_model_reset": [_vp],
     "trx_model_checkpoint": [_vp, _i],

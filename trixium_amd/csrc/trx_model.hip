@@ -18,6 +18,8 @@
 #include "trx_model.h"
 #include "trx_tgemv.h"
 #include "trx_prefill.h"
+#include "trx_attn_window.h"
+#include "trx_sample.h"
 
 namespace trx {
 
@@ -36,9 +38,10 @@ constexpr int kScoreChunk = 1024;      // and per batched prefill
 // Tokens from which the batch is faster (28 layers of the 1.7B shape, 6 of the 8B's, a period of the 27B's; ms with
 // it against one position per forward: three tokens 3.0, 1.1, 1.4 against 2.7, 0.9, 1.1; four 3.0, 1.1, 1.4
 // against 3.6, 1.3, 1.5).
-constexpr int kScoreMin = 4;
+constexpr int kRowsMin = 4;
 constexpr int kPfPartRow = 16 * 128;   // floats of K-part sums per prefill row
 constexpr int kSmpWindow = 64;
+constexpr size_t kSmpBytes = 16 + sizeof(trx_sampling);
 
 // Projections that can run on the packed GEMV (trx_tgemv.h), keyed with their layer.
 enum PackedOp { OP_QKV, OP_O, OP_GATE_UP, OP_DOWN, OP_HEAD, OP_DN_QKVZ, OP_DN_OUT };
@@ -103,11 +106,15 @@ struct Model {
   int head_S = 0, head_rows_p = 0;
   float* x2 = nullptr;                             // second residual buffer (x alternates)
   float* xrot = nullptr;                           // a rotated model's projection input
-  // Sampling (trx_model_set_sampling): temperature, top_p, repetition, then the xorshift32 state.
+  // Sampling (trx_model_set_sampling): temperature, top_p, repetition, then the xorshift32 state, then
+  // the whole vocabulary's settings (trx_model_set_vocab_sampling).
   float* smp = nullptr;
   unsigned long long* smp_cand = nullptr;          // [32] slice candidates, then the counter
   bool sampling = false;
   int smp_channels = 1;
+  bool smp_vocab = false, smp_penalty = false;     // from the whole vocabulary; with the repetition penalty
+  uint8_t* smp_work = nullptr;                     // its workspace, then the token
+  float* smp_logits = nullptr;                     // [vocab] the logits with the penalty
   float* hidden = nullptr;                         // the residual after the last layer
   // Scoring (trx_model_score): per position the normed hidden state and the next token's NLL.
   bool scoring = false;
@@ -130,6 +137,13 @@ struct Model {
   bool pf_norm = false;                            // they wait for 1 / rms(x)
   float* pf_rot = nullptr;                         // a rotated model's rotated input rows
   float* pf_rs = nullptr;                          // [pf_rows] a rotated input's 1/rms per row
+  // Prefill past the window: a chunk's K and V rows and its RoPE rows (up to pr_rows positions), and the
+  // window attention's workspace.
+  int pr_rows = 0;
+  __half *pr_k = nullptr, *pr_v = nullptr;
+  float* pr_rope = nullptr;
+  uint8_t* pr_work = nullptr;
+  size_t pr_work_bytes = 0;
   int host_n_fed = 0, host_head_from = 0;          // host copies of the control words
   hipGraph_t graph = nullptr;
   hipGraphExec_t graph_exec = nullptr;
@@ -822,7 +836,28 @@ static int run_step(Model& m, hipStream_t s) {
                           PF(m, TRX_ROLE_OUT_NORM, 0), m.logits, TRX_EPI_STORE, nullptr, s, m.slot, m.pos(),
                           m.head_from()))) return rc;
   }
-  if (m.sampling) {
+  if (m.sampling && m.smp_vocab) {
+    const float* lg = m.logits;
+    if (m.smp_penalty) {
+      PenaltyParams pp = {m.logits, m.smp_logits, c.vocab, kSmpWindow, m.pos(), m.head_from(), m.prompt(), m.prompt_ring,
+                          m.smp + 2};
+      if ((rc = launch_penalty(pp, s))) return rc;
+      lg = m.smp_logits;
+    }
+    SampleRowsParams sp = {};
+    sp.logits = lg;
+    sp.n = 1;
+    sp.vocab = c.vocab;
+    sp.ld = c.vocab;
+    sp.rows = (const trx_sampling*)(m.smp + 4);
+    sp.work = m.smp_work;
+    sp.tokens = (int32_t*)(m.smp_work + sample_rows_work_bytes(1, c.vocab));
+    sp.gate_pos = m.pos();
+    sp.gate_from = m.head_from();
+    sp.rng = (uint32_t*)(m.smp + 3);
+    sp.slot = m.slot;
+    if ((rc = launch_sample_rows(sp, s))) return rc;
+  } else if (m.sampling) {
     SampleParams sp = {m.logits, c.vocab, m.smp_channels, kSmpWindow, m.pos(), m.head_from(), m.n_prompt(),
                        m.prompt(), m.out(), c.max_new, m.smp, (uint32_t*)(m.smp + 3), m.slot, m.smp_cand,
                        (unsigned*)(m.smp_cand + 32), m.prompt_ring};
@@ -982,7 +1017,87 @@ static int pf_alloc(Model& m, int R) {
   return TRX_OK;
 }
 
+// The window attention of R positions from p0 on over the KV ring (its buffers not yet set): the pinned
+// positions and the most recent max_ctx - pin, as a decode position past the window attends.
+static AttnWindowParams ring_attention(const Model& m, int p0, int R) {
+  const trx_model_config& c = m.cfg;
+  AttnWindowParams p = {};
+  p.pos = p0;
+  p.n = R;
+  p.n_head = c.n_head;
+  p.n_kv = c.n_kv_head;
+  p.hd = c.head_dim;
+  p.slots = c.max_ctx;
+  p.pin = p.sinks = m.kv_pin;
+  p.window = c.max_ctx - m.kv_pin;
+  p.q_stride = p.out_stride = c.n_head * c.head_dim;
+  p.kv_stride = c.n_kv_head * c.head_dim;
+  p.scale = 1.f;                                     // launch_rope_kv scales q
+  if (c.attn_gated) {
+    p.gate_head_stride = 2 * c.head_dim;
+    p.gate_stride = 2 * (c.n_head + c.n_kv_head) * c.head_dim;
+  }
+  return p;
+}
+
+// The buffers of a prefill past the window in chunks of up to R positions (beside pf_alloc's). They grow
+// as those do.
+static int ring_alloc(Model& m, int R) {
+  const trx_model_config& c = m.cfg;
+  int rc;
+  if (!m.n_attn) return TRX_OK;
+  const size_t kv = (size_t)c.n_kv_head * c.head_dim * 2, rope = (size_t)(c.rope_dims ? c.rope_dims : c.head_dim) * 4;
+  if (R > m.pr_rows) {
+    int cap = 64;
+    while (cap < R) cap *= 2;
+    const std::pair<void**, size_t> bufs[] = {{(void**)&m.pr_k, kv}, {(void**)&m.pr_v, kv}, {(void**)&m.pr_rope, rope}};
+    if (m.pr_rows) TRX_HIP(hipStreamSynchronize(m.stream));
+    for (auto& b : bufs) {
+      if ((rc = dfree(m, *b.first, b.second * (size_t)m.pr_rows))) return rc;
+      *b.first = nullptr;
+    }
+    m.pr_rows = 0;
+    for (auto& b : bufs) {
+      if (!(rc = dalloc(m, b.first, b.second * (size_t)cap))) continue;
+      for (auto& f : bufs) {
+        (void)dfree(m, *f.first, f.second * (size_t)cap);
+        *f.first = nullptr;
+      }
+      return rc;
+    }
+    m.pr_rows = cap;
+  }
+  const size_t work = attn_window_work_bytes(ring_attention(m, 0, R));
+  if (work > m.pr_work_bytes) {
+    if (m.pr_work) TRX_HIP(hipStreamSynchronize(m.stream));
+    if ((rc = dfree(m, m.pr_work, m.pr_work_bytes))) return rc;
+    m.pr_work = nullptr;
+    m.pr_work_bytes = 0;
+    if ((rc = dalloc(m, (void**)&m.pr_work, work))) return rc;
+    m.pr_work_bytes = work;
+  }
+  return TRX_OK;
+}
+
+// Whether every kernel of the batched prefill takes the model in chunks of up to `chunk` positions, and
+// products of up to `widest` weight rows with it.
+static bool rows_take(const Model& m, int chunk, long long widest) {
+  const trx_model_config& c = m.cfg;
+  const int hd = c.head_dim, rope_n = c.rope_dims ? c.rope_dims : hd;
+  const int nq = c.dn_num_k_heads * c.dn_k_head_dim, nvh = c.dn_num_v_heads * c.dn_v_head_dim;
+  widest = std::max<long long>({widest, 2ll * c.ffn_dim, 2ll * c.n_head * hd + 2ll * c.n_kv_head * hd,
+                                2ll * nq + 2ll * nvh});
+  const int kmax = std::max({c.n_embd, c.ffn_dim, c.n_head * hd, nvh});
+  return widest * row_bytes_of(c.weight_kind, kmax) < (1ll << 32) && (size_t)chunk * kmax * 2 < (1ull << 32) &&
+         (!m.n_attn || attn_rows_take(c.n_head, c.n_kv_head, hd, rope_n, c.max_ctx)) &&
+         (!m.n_dn || dn_rows_take(2 * nq + nvh, c.dn_conv_kernel, c.dn_num_v_heads, c.dn_num_k_heads, c.dn_k_head_dim,
+                                  c.dn_v_head_dim));
+}
+
+// Positions p0 .. p0 + R - 1 in one pass over the weights. A chunk that ends past the window runs over the
+// KV ring.
 static int run_prefill(Model& m, int p0, int R, hipStream_t s) {
+  const bool ring = p0 + R > m.cfg.max_ctx;
   const trx_model_config& c = m.cfg;
   const int E = c.n_embd, hd = c.head_dim, F = c.ffn_dim, wk = c.weight_kind;
   const int qrows = c.n_head * hd * (c.attn_gated ? 2 : 1), kvrows = c.n_kv_head * hd;
@@ -1006,7 +1121,10 @@ static int run_prefill(Model& m, int p0, int R, hipStream_t s) {
     ep.row_bytes = row_bytes_of(c.emb_kind, E);
     ep.code_off = row_geom(c.emb_kind, E).code_off;
   }
+  ep.prompt_ring = m.prompt_ring;
   if ((rc = launch_embed_rows(ep, m.prompt(), p0, R, m.pf_x, s))) return rc;
+  if (ring && m.n_attn &&
+      (rc = launch_rope_rows(p0, R, m.rope_dev, c.rope_dims ? c.rope_dims : hd, m.pr_rope, s))) return rc;
 
   for (int l = 0; l < c.n_layer; ++l) {
     if (m.is_dn(l)) {
@@ -1067,7 +1185,25 @@ static int run_prefill(Model& m, int p0, int R, hipStream_t s) {
       rp.max_ctx = c.max_ctx;
       rp.gated = c.attn_gated;
       rp.eps = c.rms_eps;
+      if (ring) {
+        // The chunk's rows stay beside the ring until its queries have read the rows they replace.
+        rp.rope_rows = m.pr_rope;
+        rp.k_out = m.pr_k;
+        rp.v_out = m.pr_v;
+      }
       if ((rc = launch_rope_kv(rp, s))) return rc;
+      if (ring) {
+        AttnWindowParams wp = ring_attention(m, p0, R);
+        wp.q = m.pf_q;
+        wp.gate = c.attn_gated ? m.pf_qkv + hd : nullptr;
+        wp.out = m.pf_att;
+        wp.k = m.pr_k;
+        wp.v = m.pr_v;
+        wp.kcache = rp.kcache;
+        wp.vcache = rp.vcache;
+        wp.work = m.pr_work;
+        if ((rc = launch_attn_window(wp, s))) return rc;
+      }
       AttnPrefillParams ap = {};
       ap.q = m.pf_q;
       ap.qkv = m.pf_qkv;
@@ -1082,7 +1218,7 @@ static int run_prefill(Model& m, int p0, int R, hipStream_t s) {
       ap.hd = hd;
       ap.max_ctx = c.max_ctx;
       ap.gated = c.attn_gated;
-      if ((rc = launch_attn_prefill(ap, s))) return rc;
+      if (!ring && (rc = launch_attn_prefill(ap, s))) return rc;
       if ((rc = pf_prep(m, m.pf_att, c.n_head * hd, c.n_head * hd, R, nullptr, s))) return rc;
       if ((rc = pf_gemm(m, TRX_ROLE_ATTN_OUT, l, wk, E, c.n_head * hd, R, GM_RESID, m.pf_x, E, s))) return rc;
     }
@@ -1094,7 +1230,7 @@ static int run_prefill(Model& m, int p0, int R, hipStream_t s) {
   // The last position's residual is readable as the last forward's (TRX_READ_RESIDUAL), and the
   // control words move on.
   TRX_HIP(hipMemcpyAsync(m.hidden, m.pf_x + (size_t)(R - 1) * E, (size_t)E * 4, hipMemcpyDeviceToDevice, s));
-  return launch_prefill_ctl(m.pos(), m.cur_tok(), m.prompt(), p0 + R - 1, s);
+  return launch_prefill_ctl(m.pos(), m.cur_tok(), m.prompt(), m.prompt_ring, p0 + R - 1, s);
 }
 
 }  // namespace trx
@@ -1195,7 +1331,7 @@ TRX_API int trx_model_create(const trx_model_config* cfg, const float* rope_freq
   m.prompt_ring = c.max_ctx + kSmpWindow;
   if ((rc = dalloc(m, (void**)&m.ctl, (size_t)(8 + m.prompt_ring + c.max_new) * 4))) return fail(rc);
   if ((rc = dalloc(m, (void**)&m.slot, 8))) return fail(rc);
-  if ((rc = dalloc(m, (void**)&m.smp, 16))) return fail(rc);
+  if ((rc = dalloc(m, (void**)&m.smp, kSmpBytes))) return fail(rc);
   if ((rc = dalloc(m, (void**)&m.smp_cand, 33 * 8))) return fail(rc);
   TRX_HIP(hipMemset(m.smp_cand, 0, 33 * 8));
   {
@@ -1239,6 +1375,14 @@ TRX_API int trx_model_destroy(trx_model* h) {
   return TRX_OK;
 }
 
+// The captured position has (or lacks) the sampling launches asked for: it is captured again.
+static void drop_graph(Model& m) {
+  if (m.graph_exec) (void)hipGraphExecDestroy(m.graph_exec);
+  if (m.graph) (void)hipGraphDestroy(m.graph);
+  m.graph_exec = nullptr;
+  m.graph = nullptr;
+}
+
 TRX_API int trx_model_set_sampling(trx_model* h, float temperature, float top_p, float repetition,
                                    uint32_t seed, int n_channels) {
   TRX_CHECK(h && n_channels >= 1, TRX_E_INVALID, "trx_model_set_sampling: bad argument");
@@ -1251,15 +1395,34 @@ TRX_API int trx_model_set_sampling(trx_model* h, float temperature, float top_p,
   TRX_HIP(hipMemcpy(m.smp, cfg, 12, hipMemcpyHostToDevice));
   if (seed) TRX_HIP(hipMemcpy(m.smp + 3, &seed, 4, hipMemcpyHostToDevice));
   const bool on = cfg[0] > 0.f || cfg[2] > 1.f;
-  if (on != m.sampling || n_channels != m.smp_channels) {
-    // The captured position has (or lacks) the sampling launch: capture again.
-    if (m.graph_exec) (void)hipGraphExecDestroy(m.graph_exec);
-    if (m.graph) (void)hipGraphDestroy(m.graph);
-    m.graph_exec = nullptr;
-    m.graph = nullptr;
-  }
+  if (on != m.sampling || n_channels != m.smp_channels || m.smp_vocab) drop_graph(m);
   m.sampling = on;
   m.smp_channels = n_channels;
+  m.smp_vocab = false;
+  return TRX_OK;
+}
+
+TRX_API int trx_model_set_vocab_sampling(trx_model* h, float temperature, int top_k, float top_p, float min_p,
+                                         float repetition, uint32_t seed) {
+  TRX_CHECK(h, TRX_E_INVALID, "trx_model_set_vocab_sampling: null");
+  Model& m = h->m;
+  const char* why = sample_rows_refuses(1, m.cfg.vocab);
+  TRX_CHECK(!why, TRX_E_INVALID, "trx_model_set_vocab_sampling: %s", why);
+  const trx_sampling row = {temperature > 0.f ? temperature : 0.f, top_k, top_p, min_p};
+  const float rep = repetition > 1.f ? repetition : 1.f;
+  const bool penalty = rep > 1.f, on = row.temperature > 0.f || penalty;
+  int rc;
+  const size_t work = sample_rows_work_bytes(1, m.cfg.vocab);
+  if (on && !m.smp_work && (rc = dalloc(m, (void**)&m.smp_work, work + 16))) return rc;
+  if (penalty && !m.smp_logits && (rc = dalloc(m, (void**)&m.smp_logits, (size_t)m.cfg.vocab * 4))) return rc;
+  TRX_HIP(hipStreamSynchronize(m.stream));
+  TRX_HIP(hipMemcpy(m.smp + 2, &rep, 4, hipMemcpyHostToDevice));
+  TRX_HIP(hipMemcpy(m.smp + 4, &row, sizeof row, hipMemcpyHostToDevice));
+  if (seed) TRX_HIP(hipMemcpy(m.smp + 3, &seed, 4, hipMemcpyHostToDevice));
+  if (on != m.sampling || (on && (!m.smp_vocab || penalty != m.smp_penalty))) drop_graph(m);
+  m.sampling = on;
+  m.smp_vocab = on;
+  m.smp_penalty = penalty;
   return TRX_OK;
 }
 
@@ -1360,7 +1523,7 @@ static std::vector<StateRegion> state_regions(Model& m) {
   const trx_model_config& c = m.cfg;
   std::vector<StateRegion> r = {{m.ctl, (size_t)(8 + m.prompt_ring + c.max_new) * 4},
                                 {m.slot, 8},
-                                {m.smp, 16},
+                                {m.smp, kSmpBytes},
                                 {m.smp_cand, 33 * 8}};
   if (m.n_dn) {
     const int nq = c.dn_num_k_heads * c.dn_k_head_dim, nvh = c.dn_num_v_heads * c.dn_v_head_dim;
@@ -1513,19 +1676,34 @@ TRX_API int trx_model_prefill(trx_model* h, int n, int chunk) {
             m.host_head_from);
   if (n == 0) return TRX_OK;
   m.ck_lowest = std::min(m.ck_lowest, first);
-  // Positions past the window (the KV ring) run one forward each.
+  if (chunk <= 0) chunk = 1024;
+  // The positions inside the window, then the ones past it (the KV ring).
   const int n_in = std::max(0, std::min(n, m.cfg.max_ctx - first));
   if (n_in > 0) {
-    if (chunk <= 0) chunk = 1024;
-    chunk = std::min(chunk, n_in);
-    if ((rc = pf_alloc(m, chunk))) return rc;
-    for (int p0 = first; p0 < first + n_in; p0 += chunk) {
-      const int R = std::min(chunk, first + n_in - p0);
+    const int part = std::min(chunk, n_in);
+    if ((rc = pf_alloc(m, part))) return rc;
+    for (int p0 = first; p0 < first + n_in; p0 += part) {
+      const int R = std::min(part, first + n_in - p0);
       if ((rc = run_prefill(m, p0, R, m.stream))) return rc;
     }
     m.host_pos = first + n_in - 1;
   }
-  if (n_in < n) return trx_model_step(h, n - n_in, m.graph_exec != nullptr);
+  int done = n_in;
+  const int part = std::min(chunk, n - n_in);
+  if (part >= kRowsMin && rows_take(m, part, 0)) {
+    if ((rc = pf_alloc(m, part)) == TRX_OK) rc = ring_alloc(m, part);
+    const int tail = (n - n_in) % part;              // the last chunk may split its keys further
+    if (rc == TRX_OK && tail) rc = ring_alloc(m, tail);
+    if (rc != TRX_OK && rc != TRX_E_NOMEM) return rc;
+    for (; rc == TRX_OK && done < n; done += std::min(part, n - done)) {
+      const int R = std::min(part, n - done);
+      if ((rc = run_prefill(m, first + done, R, m.stream))) return rc;
+      m.host_pos = first + done + R - 1;
+    }
+  }
+  // Few of them, a shape that only the single-position kernels take, or no room for the buffers: one
+  // forward each.
+  if (done < n) return trx_model_step(h, n - done, m.graph_exec != nullptr);
   return TRX_OK;
 }
 
@@ -1577,16 +1755,7 @@ TRX_API int trx_model_generate(trx_model* h, const int32_t* prompt, int n_prompt
 // (its input's planes are in the order of the layers' code format).
 static bool score_takes(const Model& m) {
   const trx_model_config& c = m.cfg;
-  const int hd = c.head_dim, rope_n = c.rope_dims ? c.rope_dims : hd;
-  const int nq = c.dn_num_k_heads * c.dn_k_head_dim, nvh = c.dn_num_v_heads * c.dn_v_head_dim;
-  const long long widest = std::max<long long>({c.vocab, 2ll * c.ffn_dim, 2ll * c.n_head * hd + 2ll * c.n_kv_head * hd,
-                                                2ll * nq + 2ll * nvh});
-  const int kmax = std::max({c.n_embd, c.ffn_dim, c.n_head * hd, nvh});
-  return (c.head_tied ? c.emb_kind : c.head_kind) == c.weight_kind &&
-         widest * row_bytes_of(c.weight_kind, kmax) < (1ll << 32) && (size_t)kScoreChunk * kmax * 2 < (1ull << 32) &&
-         (!m.n_attn || attn_rows_take(c.n_head, c.n_kv_head, hd, rope_n, c.max_ctx)) &&
-         (!m.n_dn || dn_rows_take(2 * nq + nvh, c.dn_conv_kernel, c.dn_num_v_heads, c.dn_num_k_heads, c.dn_k_head_dim,
-                                  c.dn_v_head_dim));
+  return (c.head_tied ? c.emb_kind : c.head_kind) == c.weight_kind && rows_take(m, kScoreChunk, c.vocab);
 }
 
 // The buffers of score_batched over n positions.
@@ -1651,7 +1820,7 @@ TRX_API int trx_model_score(trx_model* h, const int32_t* tokens, int n, float* n
   // sampler draws at every position, a shape is one that only the single-position kernels take, or there is no
   // room for the batch's buffers. The last position leaves the logits and the other outputs of a forward.
   int done = 0;
-  if (n >= kScoreMin && !m.sampling && score_takes(m)) {
+  if (n >= kRowsMin && !m.sampling && score_takes(m)) {
     rc = score_alloc(m, n - 1, nll != nullptr);
     if (rc == TRX_OK) {
       if ((rc = score_batched(m, n - 1, nll != nullptr))) return rc;

@@ -18,7 +18,8 @@ struct EmbedParams {
                            // (incremented here), [5] its KV slot, [6] KV slots attended, [7] the
                            // KV ring's pinned positions (0: no ring)
   const int* n_prompt;     // device
-  const int* prompt;       // device ring of prompt_ring fed tokens (position p at p % prompt_ring)
+  int* prompt;             // device ring of prompt_ring tokens (position p at p % prompt_ring): the fed ones,
+                           // and the generated ones as they are embedded (a later feed's history)
   int prompt_ring;
   int max_ctx;             // KV slots; past them (the ring) the position's RoPE row is computed
   float* rope_cs;          // into row max_ctx of this fp32 cos|sin table (may be null)
@@ -190,7 +191,7 @@ int launch_score_rows(const ScoreRowsParams& p, hipStream_t s);
 
 int launch_embed(const EmbedParams& p, hipStream_t s);
 // Prefill: the embeddings of the tokens fed at positions p0 .. p0 + R - 1 into X [R][n_embd]
-// (p's control-word fields are not used).
+// (of p's control-word fields only prompt_ring is used).
 int launch_embed_rows(const EmbedParams& p, const int* fed, int p0, int R, float* X, hipStream_t s);
 int launch_sample(const SampleParams& p, hipStream_t s);
 int launch_finalize(const int* pos, const int* n_prompt, unsigned long long* slot, int* out, int max_out,

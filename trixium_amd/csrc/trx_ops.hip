@@ -227,6 +227,7 @@ __global__ __launch_bounds__(kEmbedThreads) void embed_kernel(EmbedParams p) {
       if (k < p.max_out) p.out[k] = tok;
     }
     if (tok < 0 || tok >= p.vocab) tok = 0;
+    if (pos >= np) p.prompt[pos % p.prompt_ring] = tok;
     *p.slot = 0ull;
     *p.cur_tok = tok;
     s_tok = tok;
@@ -244,9 +245,9 @@ __global__ __launch_bounds__(kEmbedThreads) void embed_kernel(EmbedParams p) {
   embed_token(p, s_tok, p.x);
 }
 
-// Prefill: the tokens fed at positions p0 .. p0 + gridDim.x - 1 into rows of X.
+// Prefill: the tokens fed at positions p0 .. p0 + gridDim.x - 1 (in the ring of fed tokens) into rows of X.
 __global__ __launch_bounds__(kEmbedThreads) void embed_rows_kernel(EmbedParams p, const int* fed, int p0, float* X) {
-  int tok = fed[p0 + blockIdx.x];
+  int tok = fed[(p0 + (int)blockIdx.x) % p.prompt_ring];
   if (tok < 0 || tok >= p.vocab) tok = 0;
   embed_token(p, tok, X + (size_t)blockIdx.x * p.n_embd);
 }
@@ -609,7 +610,7 @@ int launch_rotate(const RotParams& p, hipStream_t s) {
 }
 
 int launch_embed_rows(const EmbedParams& p, const int* fed, int p0, int R, float* X, hipStream_t s) {
-  TRX_CHECK(p.n_embd % kGroup == 0 && p.n_embd / kGroup <= kMaxEmbedGroups && R >= 1, TRX_E_INVALID,
+  TRX_CHECK(p.n_embd % kGroup == 0 && p.n_embd / kGroup <= kMaxEmbedGroups && R >= 1 && p.prompt_ring >= 1, TRX_E_INVALID,
             "embedding: n_embd %d unsupported", p.n_embd);
   TRX_CHECK(p.mode == EMBED_TABLE || (p.row_bytes % 16 == 0 && p.row_bytes <= kEmbedRowMax), TRX_E_INVALID,
             "embedding: row of %d bytes unsupported", p.row_bytes);

@@ -92,14 +92,20 @@ struct RopeKvParams {
   const float* rope_freq;
   const float* rope_cs;    // [max_ctx][rope_n] fp32 cos half, then sin half (or null)
   const int16_t* rope_tab;
+  const float* rope_rows;  // or the chunk's own [R][rope_n] cos and sin (launch_rope_rows; or null)
   int p0, R;
   __half* kcache;          // [n_kv][max_ctx][hd]
   __half* vcache;
+  __half* k_out;           // or, when set, the chunk's rows [R][n_kv][hd] instead of the cache
+  __half* v_out;
   float* q_out;            // [R][n_head][hd]
   int n_head, n_kv, hd, rope_n, max_ctx, gated;
   float eps;
 };
 int launch_rope_kv(const RopeKvParams& p, hipStream_t s);
+// cos and sin of the float32 angles pos * freq of positions p0 .. p0 + R - 1, each evaluated in double and
+// rounded once (as the model's table holds them): out [R][rope_n], cos half, then sin half.
+int launch_rope_rows(int p0, int R, const float* rope_freq, int rope_n, float* out, hipStream_t s);
 
 // Causal GQA attention of R query positions p0 .. p0 + R - 1 over the cache positions 0 .. each
 // query's own (fastref.py:216-241, attention_fp32:31-43): softmax(q k^T) v in fp32 from the fp16
@@ -142,7 +148,7 @@ struct DnRowsParams {
 int launch_dn_rows(const DnRowsParams& p, hipStream_t s);
 bool dn_rows_take(int C, int Kc, int nv, int nk, int hk, int hv);
 
-// Control words after a prefill of positions .. p_last: pos = p_last, cur_tok = fed[p_last].
-int launch_prefill_ctl(int* ctl_pos, int* cur_tok, const int* fed, int p_last, hipStream_t s);
+// Control words after a prefill of positions .. p_last: pos = p_last, cur_tok = fed[p_last % ring].
+int launch_prefill_ctl(int* ctl_pos, int* cur_tok, const int* fed, int ring, int p_last, hipStream_t s);
 
 }  // namespace trx

@@ -497,6 +497,9 @@ __global__ __launch_bounds__(64) void rope_kv_kernel(RopeKvParams p) {
       if (p.rope_tab) {
         cs = (float)p.rope_tab[(size_t)pos * p.rope_n + i] * (1.0f / 16384.0f);
         sn = (float)p.rope_tab[(size_t)pos * p.rope_n + half + i] * (1.0f / 16384.0f);
+      } else if (p.rope_rows) {
+        cs = p.rope_rows[(size_t)r * p.rope_n + i];
+        sn = p.rope_rows[(size_t)r * p.rope_n + half + i];
       } else if (p.rope_cs) {
         cs = p.rope_cs[(size_t)pos * p.rope_n + i];
         sn = p.rope_cs[(size_t)pos * p.rope_n + half + i];
@@ -512,18 +515,37 @@ __global__ __launch_bounds__(64) void rope_kv_kernel(RopeKvParams p) {
 #pragma unroll
     for (int e = 0; e < E; ++e) dst[lane + 64 * e] = o[e] * post;
   } else {
-    const size_t c = ((size_t)g * p.max_ctx + pos) * HD;
+    const size_t c = p.k_out ? ((size_t)r * p.n_kv + g) * HD : ((size_t)g * p.max_ctx + pos) * HD;
+    __half* kd = p.k_out ? p.k_out : p.kcache;
+    __half* vd = p.k_out ? p.v_out : p.vcache;
     const float* vsrc = p.qkv + (size_t)r * p.ldq + (size_t)p.n_head * qstride + (size_t)p.n_kv * HD + (size_t)g * HD;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      p.kcache[c + lane + 64 * e] = __float2half(o[e]);
-      p.vcache[c + lane + 64 * e] = __float2half(vsrc[lane + 64 * e]);
+      kd[c + lane + 64 * e] = __float2half(o[e]);
+      vd[c + lane + 64 * e] = __float2half(vsrc[lane + 64 * e]);
     }
   }
 }
 
+__global__ void rope_rows_kernel(int p0, const float* rope_freq, int rope_n, float* out) {
+  const int half = rope_n / 2, i = threadIdx.x;
+  if (i >= half) return;
+  const double ang = (double)((float)(p0 + (int)blockIdx.x) * rope_freq[i]);
+  float* row = out + (size_t)blockIdx.x * rope_n;
+  row[i] = (float)cos(ang);
+  row[half + i] = (float)sin(ang);
+}
+
+int launch_rope_rows(int p0, int R, const float* rope_freq, int rope_n, float* out, hipStream_t s) {
+  TRX_CHECK(R >= 1 && p0 >= 0 && rope_n >= 2 && rope_n <= 2048 && rope_n % 2 == 0, TRX_E_INVALID,
+            "prefill RoPE: %d rows of %d", R, rope_n);
+  hipLaunchKernelGGL(rope_rows_kernel, dim3(R), dim3((rope_n / 2 + 63) / 64 * 64), 0, s, p0, rope_freq, rope_n, out);
+  TRX_LAUNCHED();
+  return TRX_OK;
+}
+
 int launch_rope_kv(const RopeKvParams& p, hipStream_t s) {
-  TRX_CHECK(p.R >= 1 && p.p0 >= 0 && p.p0 + p.R <= p.max_ctx && p.rope_n % 2 == 0 && p.rope_n <= p.hd,
+  TRX_CHECK(p.R >= 1 && p.p0 >= 0 && (p.k_out ? p.v_out && p.rope_rows : p.p0 + p.R <= p.max_ctx) && p.rope_n % 2 == 0 && p.rope_n <= p.hd,
             TRX_E_INVALID, "prefill RoPE: positions %d..%d", p.p0, p.p0 + p.R);
   const dim3 grid(p.R, p.n_head + p.n_kv);
   if (p.hd == 64) hipLaunchKernelGGL(rope_kv_kernel<64>, grid, dim3(64), 0, s, p);
@@ -1119,15 +1141,15 @@ int launch_dn_rows(const DnRowsParams& p, hipStream_t s) {
   return TRX_OK;
 }
 
-__global__ void prefill_ctl_kernel(int* ctl_pos, int* cur_tok, const int* fed, int p_last) {
+__global__ void prefill_ctl_kernel(int* ctl_pos, int* cur_tok, const int* fed, int ring, int p_last) {
   if (threadIdx.x == 0 && blockIdx.x == 0) {
     *ctl_pos = p_last;
-    *cur_tok = fed[p_last];
+    *cur_tok = fed[p_last % ring];
   }
 }
 
-int launch_prefill_ctl(int* ctl_pos, int* cur_tok, const int* fed, int p_last, hipStream_t s) {
-  hipLaunchKernelGGL(prefill_ctl_kernel, dim3(1), dim3(64), 0, s, ctl_pos, cur_tok, fed, p_last);
+int launch_prefill_ctl(int* ctl_pos, int* cur_tok, const int* fed, int ring, int p_last, hipStream_t s) {
+  hipLaunchKernelGGL(prefill_ctl_kernel, dim3(1), dim3(64), 0, s, ctl_pos, cur_tok, fed, ring, p_last);
   TRX_LAUNCHED();
   return TRX_OK;
 }

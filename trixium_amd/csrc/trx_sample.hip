@@ -42,6 +42,7 @@ struct SrState {
   u64 cut;                     // tokens below this (logit, index) are out
   u64 base;                    // EDGE: count or mass before the gathered step
   u64 total;                   // mass of every live token
+  float u;
 };
 
 // The workspace of a row, in this order.
@@ -281,15 +282,37 @@ __device__ __forceinline__ void sr_extremes(const SrWork& w, int chunks, u64* re
 
 __device__ __forceinline__ bool sr_none(u64 top) { return sr_logit(top) == -INFINITY; }
 
+// A decode position that computes no logits draws nothing.
+__device__ __forceinline__ bool sr_gated(const SampleRowsParams& p) { return p.gate_pos && *p.gate_pos < *p.gate_from; }
+
+__device__ __forceinline__ void sr_put(const SampleRowsParams& p, int row, int token, float logp) {
+  p.tokens[row] = token;
+  if (p.logp) p.logp[row] = logp;
+  if (p.slot) *p.slot = (1ull << 32) | (u64)(0xFFFFFFFFu - (uint32_t)max(token, 0));
+}
+
 // 1. Every chunk's largest token and smallest logit; the row's histogram and state cleared.
 template <class T>
 __global__ __launch_bounds__(kSrThreads) void sample_extremes_kernel(SampleRowsParams p) {
   __shared__ u64 red[4];
   __shared__ float lred[4];
+  if (sr_gated(p)) return;
   const int row = blockIdx.x / p.chunks, c = blockIdx.x - row * p.chunks, t = threadIdx.x;
   const SrWork w = sr_work(p.work, row);
   for (int i = c * kSrThreads + t; i < kSrBuckets; i += p.chunks * kSrThreads) w.hmass[i] = 0, w.hcount[i] = 0;
-  if (c == 0 && t == 0) *w.st = SrState{SR_DONE, 0, 0, 0, 0, 0, 0};
+  if (c == 0 && t == 0) {
+    *w.st = SrState{SR_DONE, 0, 0, 0, 0, 0, 0, 0.f};
+    if (!p.rng) {
+      w.st->u = p.u[row];
+    } else if (!sr_row(p, row).greedy) {
+      uint32_t x = *p.rng;
+      x ^= x << 13;
+      x ^= x >> 17;
+      x ^= x << 5;
+      *p.rng = x;
+      w.st->u = (float)(x >> 8) * (1.0f / 16777216.0f);
+    }
+  }
   const SrLogits<T> lg(p, row);
   u64 top = 0;
   float low = INFINITY;
@@ -318,6 +341,7 @@ __global__ __launch_bounds__(kSrThreads) void sample_histogram_kernel(SampleRows
   __shared__ u64 hm[kSrBuckets];
   __shared__ uint32_t hc[kSrBuckets];
   __shared__ u64 red[4];
+  if (sr_gated(p)) return;
   const int row = blockIdx.x / p.chunks, c = blockIdx.x - row * p.chunks, t = threadIdx.x;
   const SrWork w = sr_work(p.work, row);
   const SrRow s = sr_row(p, row);
@@ -326,8 +350,8 @@ __global__ __launch_bounds__(kSrThreads) void sample_histogram_kernel(SampleRows
   sr_extremes(w, p.chunks, red, top, low);
   if (s.greedy || sr_none(top)) {
     if (c == 0 && t == 0) {
-      p.tokens[row] = sr_none(top) ? -1 : sr_index(top);
-      if (p.logp) p.logp[row] = sr_none(top) ? NAN : 0.f;
+      if (sr_none(top)) sr_put(p, row, -1, NAN);
+      else sr_put(p, row, sr_index(top), 0.f);
     }
     return;
   }
@@ -416,6 +440,7 @@ __device__ SrPlan sr_plan(const SrWork& w, const SrRow& s, u64* red) {
 template <class T>
 __global__ __launch_bounds__(kSrThreads) void sample_gather_kernel(SampleRowsParams p) {
   __shared__ u64 red[4];
+  if (sr_gated(p)) return;
   const int row = blockIdx.x / p.chunks, c = blockIdx.x - row * p.chunks, t = threadIdx.x;
   const SrWork w = sr_work(p.work, row);
   const SrRow s = sr_row(p, row);
@@ -469,10 +494,8 @@ __device__ u64 sr_select(Each each, u64 want, int bits, u64* hist, u64* red) {
 
 __device__ __forceinline__ void sr_store(const SampleRowsParams& p, int row, const SrScale& sc, float T, float l, int i,
                                          u64 total) {
-  p.tokens[row] = i;
-  if (!p.logp) return;
   const double d = sc.inf ? 0.0 : -(sc.top - (double)l) / (double)T;
-  p.logp[row] = (float)(d - log(ldexp((double)total, -sc.frac)));
+  sr_put(p, row, i, p.logp ? (float)(d - log(ldexp((double)total, -sc.frac))) : 0.f);
 }
 
 // 4. A block a row: the cut, and the draw where every token that stayed was gathered.
@@ -480,6 +503,7 @@ template <class T>
 __global__ __launch_bounds__(kSrRowThreads) void sample_cut_kernel(SampleRowsParams p) {
   __shared__ u64 key_s[kSrGather], mass_s[kSrGather];
   __shared__ u64 hist[256], red[16];
+  if (sr_gated(p)) return;
   const int row = blockIdx.x, t = threadIdx.x;
   const SrWork w = sr_work(p.work, row);
   const SrState st = *w.st;
@@ -556,7 +580,7 @@ __global__ __launch_bounds__(kSrRowThreads) void sample_cut_kernel(SampleRowsPar
   auto by_index = [&](auto f) {
     for (int i = t; i < n; i += kSrRowThreads) f(key_s[i] & (kSrMaxVocab - 1), mass_s[i]);
   };
-  const u64 pick = sr_select(by_index, sr_target(p.u[row], total) + 1, 24, hist, red);
+  const u64 pick = sr_select(by_index, sr_target(st.u, total) + 1, 24, hist, red);
   for (int i = t; i < n; i += kSrRowThreads)
     if (mass_s[i] && (key_s[i] & (kSrMaxVocab - 1)) == pick) sr_store(p, row, sc, s.temperature, sr_logit(key_s[i]), sr_index(pick), total);
   if (t == 0) w.st->mode = SR_DONE;
@@ -566,6 +590,7 @@ __global__ __launch_bounds__(kSrRowThreads) void sample_cut_kernel(SampleRowsPar
 template <class T>
 __global__ __launch_bounds__(kSrThreads) void sample_mass_kernel(SampleRowsParams p) {
   __shared__ u64 red[4];
+  if (sr_gated(p)) return;
   const int row = blockIdx.x / p.chunks, c = blockIdx.x - row * p.chunks, t = threadIdx.x;
   const SrWork w = sr_work(p.work, row);
   if (w.st->mode != SR_DRAW) return;
@@ -590,6 +615,7 @@ template <class T>
 __global__ __launch_bounds__(kSrRowThreads) void sample_draw_kernel(SampleRowsParams p) {
   __shared__ u64 red[16], before_s;
   __shared__ int chunk_s;
+  if (sr_gated(p)) return;
   const int row = blockIdx.x, t = threadIdx.x;
   const SrWork w = sr_work(p.work, row);
   if (w.st->mode != SR_DRAW) return;
@@ -602,7 +628,7 @@ __global__ __launch_bounds__(kSrRowThreads) void sample_draw_kernel(SampleRowsPa
   const u64 least = sc.floor_mass(s.min_p);
   const u64 mc = t < p.chunks ? w.mass[t] : 0;
   const u64 total = block_sum_u64(mc, red);
-  u64 want = sr_target(p.u[row], total);
+  u64 want = sr_target(w.st->u, total);
   const u64 bc = block_before_u64(mc, red);
   if (bc <= want && want < bc + mc) chunk_s = t, before_s = bc;
   __syncthreads();
@@ -630,6 +656,31 @@ __global__ __launch_bounds__(kSrRowThreads) void sample_draw_kernel(SampleRowsPa
     if (want < all) return;
     want -= all;
   }
+}
+
+// The repetition penalty --------------------------------------------------------------------------
+
+constexpr int kPenaltyWindow = 64;          // positions at most (a thread each)
+
+__global__ __launch_bounds__(kSrThreads) void penalty_kernel(PenaltyParams p) {
+  const int pos = *p.pos;
+  if (pos < *p.head_from) return;
+  const int t = threadIdx.x, i0 = blockIdx.x * kSrChunk, i1 = min(p.vocab, i0 + kSrChunk);
+  for (int i = i0 + t; i < i1; i += kSrThreads) p.out[i] = p.logits[i];
+  __syncthreads();                           // the block's own copies first
+  const int j = pos - t;
+  if (t >= min(p.window, kPenaltyWindow) || j < 0) return;
+  const int tok = p.tokens[j % p.ring];
+  if (tok < i0 || tok >= i1) return;
+  const float v = p.logits[tok], rep = *p.repetition;
+  p.out[tok] = v > 0.f ? v / rep : v * rep;  // of a token that stands twice, twice the same value
+}
+
+int launch_penalty(const PenaltyParams& p, hipStream_t s) {
+  TRX_CHECK(p.vocab > 0 && p.window >= 0 && p.window <= kPenaltyWindow, TRX_E_INVALID, "penalty: bad parameters");
+  hipLaunchKernelGGL(penalty_kernel, dim3(cdiv(p.vocab, kSrChunk)), dim3(kSrThreads), 0, s, p);
+  TRX_LAUNCHED();
+  return TRX_OK;
 }
 
 // Launch ------------------------------------------------------------------------------------------

@@ -281,6 +281,15 @@ class Decoder:
         _lib.call("trx_model_set_sampling", self._h, float(temperature), float(top_p), float(repetition),
                   int(seed) & 0xFFFFFFFF, n)
 
+    def set_vocab_sampling(self, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, repetition=1.0, seed=0):
+        """Sample from the whole vocabulary (trx_model_set_vocab_sampling): the repetition penalty over the
+        last 64 tokens, temperature, the top_k largest, the smallest prefix holding top_p, at least min_p of
+        the largest probability (0, 1 and 0 are off), one number of the firmware's xorshift32 stream a token
+        (seed 0 keeps it). set_sampling's firmware sampler draws among 32 candidates; the last of the two
+        calls counts, and set_sampling() is the greedy argmax again."""
+        _lib.call("trx_model_set_vocab_sampling", self._h, float(temperature), int(top_k), float(top_p), float(min_p),
+                  float(repetition), int(seed) & 0xFFFFFFFF)
+
     # State and decoding ------------------------------------------------------------------------
     def reset(self):
         _lib.call("trx_model_reset", self._h)
