@@ -37,6 +37,7 @@ constexpr float kLog2e = 1.44269504088896341f;
 typedef _Float16 half2v_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 
 // LDS row strides in halves. K rows are read 16 bytes a lane, a row a lane: one 16-byte step a row
@@ -146,33 +147,30 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ * WK / 4) void attn_window_kernel(
   const int srow = tid / SEG, sd = (tid % SEG) * 8;
   const int R = p.slots - p.pin, ub = max(lo, p.pin);
   const int roff = (int)((unsigned)(ub - p.pin) % (unsigned)R);   // ring offset of position ub
-  const __half* kc = p.kcache + (size_t)g * p.slots * HD + sd;
-  const __half* vc = p.vcache + (size_t)g * p.slots * HD + sd;
-  const __half* kn = p.k + g * HD + sd;
-  const __half* vn = p.v + g * HD + sd;
-  uint4 kr[PP], vr[PP];
+  const char* const kc = (const char*)(p.kcache + (size_t)g * p.slots * HD + sd);
+  const char* const vc = (const char*)(p.vcache + (size_t)g * p.slots * HD + sd);
+  // The call's own rows as distances from the ring's: one address a load, whichever side it reads.
+  const long long kd = (const char*)(p.k + g * HD + sd) - kc, vd = (const char*)(p.v + g * HD + sd) - vc;
+  u32x4_t kr[PP], vr[PP];
   auto load = [&](int st) {
 #pragma unroll
     for (int i = 0; i < PP; ++i) {
       // Past the last key: that key again (masked).
       const int x = min(st * SR + srow + i * RPP, N - 1);
       const int u = x < ns ? x : x - ns + lo;
-      int slot = u;
-      if (u >= p.pin) {
-        slot = roff + (u - ub);                   // u - ub < window <= R
-        slot = p.pin + (slot >= R ? slot - R : slot);
-      }
-      const bool old = u < pos;
-      const size_t off = old ? (size_t)slot * HD : (size_t)(u - pos) * p.kv_stride;
-      kr[i] = *(const uint4*)((old ? kc : kn) + off);
-      vr[i] = *(const uint4*)((old ? vc : vn) + off);
+      const int ro = roff + (u - ub);               // u - ub < window <= R
+      const int slot = u < p.pin ? u : p.pin + (ro >= R ? ro - R : ro);
+      const int fresh = u < pos ? 0 : -1;
+      const long long at = 2ll * (fresh ? u - pos : slot) * (fresh ? p.kv_stride : HD);
+      kr[i] = *(const u32x4_t*)(kc + at + (kd & (long long)fresh));
+      vr[i] = *(const u32x4_t*)(vc + at + (vd & (long long)fresh));
     }
   };
   auto store = [&](int buf) {
 #pragma unroll
     for (int i = 0; i < PP; ++i) {
-      *(uint4*)(ks + buf * KB + (srow + i * RPP) * KS + sd) = kr[i];
-      *(uint4*)(vs + buf * VB + (srow + i * RPP) * VS + sd) = vr[i];
+      *(u32x4_t*)(ks + buf * KB + (srow + i * RPP) * KS + sd) = kr[i];
+      *(u32x4_t*)(vs + buf * VB + (srow + i * RPP) * VS + sd) = vr[i];
     }
   };
 
