@@ -217,13 +217,13 @@ int trx_gemv_packed_parts_f32(const uint8_t* packed, int kind, int M, int K, con
  * r * q_stride + h * head_dim, of out at r * out_stride + h * head_dim, of gate at r * gate_stride +
  * h * gate_head_stride; row r of k and v (fp16, post-RoPE, position pos + r) has kv head g at
  * r * kv_stride + g * head_dim. Strides are in elements: q_stride a multiple of 16 bytes, kv_stride of
- * 8, the others of 4; every pointer is 16-byte aligned.
+ * 8 and at most 2^22, the others of 4; every pointer is 16-byte aligned.
  * head_dim 64, 128 or 256; 0 <= sinks <= pin < slots, 1 <= window <= slots - pin, scale > 0, n >= 0
  * (0: nothing is done).
  * The ring holds the positions below pos that a query sees; slots that no visible position takes may
  * hold anything. Afterwards the new rows stand in their slots (of rows that share a slot, the last);
  * no other slot is written. An infinity or NaN in a key or value that a query does not see does not
- * reach its output. out, workspace and the ring overlap no other argument.
+ * reach its output; one in a value that it sees makes that element infinite or NaN. out, workspace and the ring overlap no other argument.
  * pos_dev != NULL: the first position is read from the device when the work runs (for captured
  * graphs) and `pos` is ignored; a position there that is negative or leaves int32 within n leaves out
  * and the ring as they are.
