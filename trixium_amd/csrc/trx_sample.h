@@ -26,6 +26,7 @@ struct SampleRowsParams {
   unsigned long long* slot;
   // Set by the launcher.
   int chunk, chunks, frac;     // logits a block; blocks a row; fractional bits of a mass
+  int part, parts;             // logits a part of a chunk; parts a chunk
 };
 
 const char* sample_rows_refuses(int n, int vocab);

@@ -13,9 +13,14 @@
 //
 // No sort of the vocabulary: a histogram over 1024 steps of the logit's distance from the largest
 // (counts and masses) finds the step that the cut falls into; the tokens of that step, or with a short
-// list every token up to it, are gathered, and the cut is found among them by eight bits of (logit,
+// list every token up to it, are gathered, and the cut is found among them by nine bits of (logit,
 // index) at a time. A row whose cut step holds more than a block gathers (many equal or nearly equal
 // logits) is cut by the same rounds over the row itself.
+//
+// What bounds it: many rows, reading them (the largest logits, the histogram, the gather; for a row drawn from more
+// than was gathered, the masses) and the 64-bit exponentials; a single row, six launches that wait for each other.
+// us per launch, 160 rows of 248320 fp32 logits (159 MB) with top_p: 28 (5.7 TB/s), 61 (without the
+// exponentials 42), 41, the cuts 20, masses 20, draws 10; one row of 151936: 4, 7, 7, 11, 1 to 4, 1.
 
 #include "trx_sample.h"
 
@@ -25,10 +30,14 @@ namespace trx {
 
 constexpr int kSrBuckets = 1024;
 constexpr int kSrGather = 4096;             // tokens a row's gather holds
+constexpr int kSrBlockGather = 1024;        // of a block's, before it counts them into the row's
 constexpr int kSrThreads = 256;             // of the kernels that stream a row
 constexpr int kSrChunk = 4096;              // logits a block, at least
 constexpr int kSrChunksMax = 256;
-constexpr int kSrRowThreads = 1024;         // of the kernels with a block a row
+constexpr int kSrBlocks = 2048;
+constexpr int kSrChunkParts = 16;           // of a chunk at most
+constexpr int kSrRowThreads = 512;          // of the kernels with a block a row
+constexpr int kSrParts = kSrRowThreads;     // of a row, whose masses the draw's block looks through
 constexpr int kSrMaxVocab = 1 << 24;        // an index takes 24 bits beside the logit's 32
 
 typedef unsigned long long u64;
@@ -48,7 +57,7 @@ struct SrState {
 // The workspace of a row, in this order.
 struct SrWork {
   u64* top;                    // [chunks] each chunk's largest (logit, index)
-  u64* mass;                   // [chunks] mass that stayed
+  u64* mass;                   // [kSrParts] mass that stayed
   u64* hmass;                  // [kSrBuckets]
   u64* item;                   // [kSrGather] gathered tokens
   SrState* st;
@@ -56,7 +65,7 @@ struct SrWork {
   float* low;                  // [chunks] each chunk's smallest logit above -inf
 };
 constexpr size_t sr_row_bytes() {
-  return (size_t)kSrChunksMax * 16 + (size_t)kSrBuckets * 8 + (size_t)kSrGather * 8 + sizeof(SrState) +
+  return (size_t)(kSrChunksMax + kSrParts) * 8 + (size_t)kSrBuckets * 8 + (size_t)kSrGather * 8 + sizeof(SrState) +
          (size_t)kSrBuckets * 4 + (size_t)kSrChunksMax * 4;
 }
 __device__ __forceinline__ SrWork sr_work(void* work, int row) {
@@ -64,7 +73,7 @@ __device__ __forceinline__ SrWork sr_work(void* work, int row) {
   SrWork w;
   w.top = (u64*)b;
   w.mass = w.top + kSrChunksMax;
-  w.hmass = w.mass + kSrChunksMax;
+  w.hmass = w.mass + kSrParts;
   w.item = w.hmass + kSrBuckets;
   w.st = (SrState*)(w.item + kSrGather);
   w.hcount = (uint32_t*)(w.st + 1);
@@ -116,31 +125,55 @@ struct SrScale {
     per = !inf && reach > 0.0 ? kSrBuckets / reach : 0.0;
   }
   __device__ __forceinline__ u64 mass(float l) const {
-    if (inf) return l == INFINITY ? 1ull << frac : 0;
-    const double y = -(top - (double)l) * c2;
-    if (!(y >= -(double)(frac + 1))) return 0;
-    // 2^y = 2^n e^(f ln 2), |f| <= 1/2: the series to the twelfth power is off by 2^-52.
-    const double n = rint(y), f = (y - n) * 0.69314718055994530942;
-    double w = 1.0 / 479001600.0;
-    w = fma(w, f, 1.0 / 39916800.0);
-    w = fma(w, f, 1.0 / 3628800.0);
-    w = fma(w, f, 1.0 / 362880.0);
-    w = fma(w, f, 1.0 / 40320.0);
-    w = fma(w, f, 1.0 / 5040.0);
-    w = fma(w, f, 1.0 / 720.0);
-    w = fma(w, f, 1.0 / 120.0);
-    w = fma(w, f, 1.0 / 24.0);
-    w = fma(w, f, 1.0 / 6.0);
-    w = fma(w, f, 0.5);
-    w = fma(w, f, 1.0);
-    w = fma(w, f, 1.0);
-    // Rounded to an integer below 2^52 by the addition of 2^52.
-    const double v = ldexp(w, (int)n + frac) + 4503599627370496.0;
-    return (u64)__double_as_longlong(v) & 0xFFFFFFFFFFFFFull;
+    u64 m;
+    masses<1>(&l, &m);
+    return m;
+  }
+  // Of N logits side by side, their chains of products interleaved and without branches: one logit after the
+  // other took twice as long.
+  template <int N>
+  __device__ __forceinline__ void masses(const float* l, u64* m) const {
+    if (inf) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) m[i] = l[i] == INFINITY ? 1ull << frac : 0;
+      return;
+    }
+    // 2^y = 2^n 2^f, |f| <= 1/2: the series of e^(f ln 2) to the twelfth power is off by 2^-52.
+    constexpr double k1 = 0.69314718055994530942, k2 = k1 * k1 / 2, k3 = k2 * k1 / 3, k4 = k3 * k1 / 4, k5 = k4 * k1 / 5,
+                     k6 = k5 * k1 / 6, k7 = k6 * k1 / 7, k8 = k7 * k1 / 8, k9 = k8 * k1 / 9, k10 = k9 * k1 / 10,
+                     k11 = k10 * k1 / 11, k12 = k11 * k1 / 12;
+    constexpr double k[12] = {k11, k10, k9, k8, k7, k6, k5, k4, k3, k2, k1, 1.0};
+    double f[N], w[N];
+    int n[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const double y = fmax(((double)l[i] - top) * c2, -(double)(frac + 2));   // below: 0 as well
+      const double t = y + 6755399441055744.0;  // 1.5 2^52: y rounded, in the low bits
+      n[i] = (int)__double_as_longlong(t);
+      f[i] = y - (t - 6755399441055744.0);
+      w[i] = k12;
+    }
+#pragma unroll
+    for (int j = 0; j < 12; ++j)
+#pragma unroll
+      for (int i = 0; i < N; ++i) w[i] = fma(w[i], f[i], k[j]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      // Times 2^(n + frac) on the exponent; rounded to an integer below 2^52 by the addition of 2^52 (a quarter
+      // and a half go to 0).
+      const double x = __longlong_as_double(__double_as_longlong(w[i]) + ((long long)(n[i] + frac) << 52));
+      m[i] = (u64)__double_as_longlong(x + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
+    }
   }
   __device__ __forceinline__ int bucket(float l) const {
-    return min(kSrBuckets - 1, (int)fmin((top - (double)l) * per, (double)kSrBuckets));
+    return (int)fminf((float)(((double)l - top) * -per), (float)(kSrBuckets - 1));
   }
+  // Not above any logit of the buckets up to b (half a bucket of slack, then the float next to it).
+  __device__ __forceinline__ float under(int b) const {
+    return b >= kSrBuckets - 1 || !(per > 0.0) ? -INFINITY : (float)(top - (b + 1.5) / per);
+  }
+  // Not below any logit of the buckets from b on.
+  __device__ __forceinline__ float over(int b) const { return (float)(top - (b - 0.5) / per); }
   // The smallest mass that min_p lets stay.
   __device__ __forceinline__ u64 floor_mass(float min_p) const {
     return (u64)ceil(ldexp((double)min_p, frac));
@@ -186,31 +219,55 @@ struct SrLogits {
   __device__ __forceinline__ float at(int i) const { return sr_clean((float)row[i]); }
   __device__ __forceinline__ int begin(int c, int chunk) const { return c ? min(vocab, head + c * chunk) : 0; }
   __device__ __forceinline__ int end(int c, int chunk) const { return (int)min((long long)vocab, head + (c + 1ll) * chunk); }
-  // f(logit, index) for every element of chunk c, over the block's threads.
   template <int THREADS, class F>
   __device__ __forceinline__ void each(int c, int chunk, F f) const {
-    if (c == 0 && (int)threadIdx.x < head) f(at(threadIdx.x), (int)threadIdx.x);
-    const int e1 = end(c, chunk);
-    constexpr int U = 4;
-    for (int i0 = head + c * chunk + (int)threadIdx.x * E; i0 < e1; i0 += THREADS * E * U) {
-      uint4 raw[U];
+    span<THREADS>(c * chunk, end(c, chunk), f, [] {});
+  }
+  // f(logits, index of the first) for every piece of E elements from the first-th behind the head on (0: the head
+  // too) to before e1, over the block's threads; what a piece lacks is -inf. Four pieces a thread are on their way
+  // while four are worked on; group() follows each four, in every thread.
+  static constexpr int U = 4;
+  template <int THREADS, class F, class G>
+  __device__ __forceinline__ void span(int first, int e1, F f, G group) const {
+    constexpr int S = THREADS * E * U;
+    if (first == 0 && (int)threadIdx.x < head) {
+      float v[E];
+#pragma unroll
+      for (int x = 1; x < E; ++x) v[x] = -INFINITY;
+      v[0] = at(threadIdx.x);
+      f(v, (int)threadIdx.x);
+    }
+    uint4 raw[U];
+    auto load = [&](uint4* to, int g) __attribute__((always_inline)) {
 #pragma unroll
       for (int k = 0; k < U; ++k) {
-        const int i = i0 + k * THREADS * E;
-        if (i + E <= e1) raw[k] = *(const uint4*)(row + i);
+        const int i = g + (k * THREADS + (int)threadIdx.x) * E;
+        if (i + E <= e1) to[k] = *(const uint4*)(row + i);
       }
+    };
+    load(raw, head + first);
+    for (int g = head + first; g < e1; g += S) {
+      uint4 next[U];
+      if (g + S < e1) load(next, g + S);
 #pragma unroll
       for (int k = 0; k < U; ++k) {
-        const int i = i0 + k * THREADS * E;
+        const int i = g + (k * THREADS + (int)threadIdx.x) * E;
+        if (i >= e1) break;
+        float v[E];
         if (i + E <= e1) {
-          T v[E];
-          __builtin_memcpy(v, &raw[k], 16);
+          T x[E];
+          __builtin_memcpy(x, &raw[k], 16);
 #pragma unroll
-          for (int x = 0; x < E; ++x) f(sr_clean((float)v[x]), i + x);
+          for (int j = 0; j < E; ++j) v[j] = sr_clean((float)x[j]);
         } else {
-          for (int x = i; x < e1; ++x) f(at(x), x);
+#pragma unroll
+          for (int j = 0; j < E; ++j) v[j] = i + j < e1 ? at(i + j) : -INFINITY;
         }
+        f(v, i);
       }
+      group();
+#pragma unroll
+      for (int k = 0; k < U; ++k) raw[k] = next[k];
     }
   }
 };
@@ -224,61 +281,78 @@ __device__ __forceinline__ u64 wave_max_u64(u64 v) {
   return v;
 }
 __device__ __forceinline__ float wave_min(float v) { return -wave_max(-v); }
-__device__ __forceinline__ u64 wave_sum_u64(u64 v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+// The sum of this lane's value and those of the lanes before it: rows of 16 by shifts, then the rows' ends.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp_u64(u64 v) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, true);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xF, true);
+  return (u64)hi << 32 | lo;
+}
+__device__ __forceinline__ u64 wave_upto_u64(u64 v) {
+  v += dpp_u64<0x111, 0xF>(v);                 // row_shr 1, 2, 4, 8
+  v += dpp_u64<0x112, 0xF>(v);
+  v += dpp_u64<0x114, 0xF>(v);
+  v += dpp_u64<0x118, 0xF>(v);
+  v += dpp_u64<0x142, 0xA>(v);                 // row_bcast 15 into rows 1 and 3
+  v += dpp_u64<0x143, 0xC>(v);                 // row_bcast 31 into rows 2 and 3
   return v;
 }
-// Sum over the block (every thread gets it); red holds a value a wave.
+// Sum over the block (every thread gets it); red holds a value a wave, of 16 at most.
 __device__ __forceinline__ u64 block_sum_u64(u64 v, u64* red) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
-  v = wave_sum_u64(v);
+  v = wave_upto_u64(v);
   __syncthreads();
-  if (lane == 0) red[w] = v;
+  if (lane == 63) red[w] = v;
   __syncthreads();
   u64 t = 0;
-  for (int i = 0; i < nw; ++i) t += red[i];
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (i < nw) t += red[i];
   return t;
 }
 // Sum of the values of the threads before this one.
 __device__ __forceinline__ u64 block_before_u64(u64 v, u64* red) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  u64 x = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const u64 y = __shfl_up(x, o, 64);
-    if (lane >= o) x += y;
-  }
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
+  const u64 x = wave_upto_u64(v);
   __syncthreads();
   if (lane == 63) red[w] = x;
   __syncthreads();
   u64 t = 0;
-  for (int i = 0; i < w; ++i) t += red[i];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const u64 r = i < nw ? red[i] : 0;
+    t += i < w ? r : 0;
+  }
   return t + x - v;
 }
 
-// The row's largest (logit, index) and smallest logit from its chunks' (every thread gets them).
-__device__ __forceinline__ void sr_extremes(const SrWork& w, int chunks, u64* red, u64& top, float& low) {
-  u64 t = 0;
-  float l = INFINITY;
-  for (int i = threadIdx.x; i < chunks; i += blockDim.x) {
-    t = w.top[i] > t ? w.top[i] : t;
-    l = fminf(l, w.low[i]);
+// The row's largest (logit, index) and smallest logit from its chunks' (every thread gets them): the thread's
+// share first, so that a kernel's first loads are on their way together.
+struct SrExtremes {
+  u64 t;
+  float l;
+  __device__ __forceinline__ SrExtremes(const SrWork& w, int chunks) : t(0), l(INFINITY) {
+    for (int i = threadIdx.x; i < chunks; i += blockDim.x) {
+      t = w.top[i] > t ? w.top[i] : t;
+      l = fminf(l, w.low[i]);
+    }
   }
-  t = wave_max_u64(t);
-  l = wave_min(l);
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, nw = blockDim.x >> 6;
-  __shared__ float lred[16];
-  __syncthreads();
-  if (lane == 0) red[wv] = t, lred[wv] = l;
-  __syncthreads();
-  for (int i = 0; i < nw; ++i) {
-    t = red[i] > t ? red[i] : t;
-    l = fminf(l, lred[i]);
+  __device__ __forceinline__ void get(u64* red, u64& top, float& low) {
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, nw = min((int)blockDim.x, kSrChunksMax) >> 6;
+    t = wave_max_u64(t);
+    l = wave_min(l);
+    __shared__ float lred[16];
+    __syncthreads();
+    if (lane == 0) red[wv] = t, lred[wv] = l;
+    __syncthreads();
+    for (int i = 0; i < nw; ++i) {             // (no chunk's thread is in a later wave)
+      t = red[i] > t ? red[i] : t;
+      l = fminf(l, lred[i]);
+    }
+    top = t;
+    low = l;
   }
-  top = t;
-  low = l;
-}
+};
 
 __device__ __forceinline__ bool sr_none(u64 top) { return sr_logit(top) == -INFINITY; }
 
@@ -301,7 +375,7 @@ __global__ __launch_bounds__(kSrThreads) void sample_extremes_kernel(SampleRowsP
   const SrWork w = sr_work(p.work, row);
   for (int i = c * kSrThreads + t; i < kSrBuckets; i += p.chunks * kSrThreads) w.hmass[i] = 0, w.hcount[i] = 0;
   if (c == 0 && t == 0) {
-    *w.st = SrState{SR_DONE, 0, 0, 0, 0, 0, 0, 0.f};
+    *w.st = SrState{sr_row(p, row).cut ? SR_DONE : SR_DRAW, 0, 0, 0, 0, 0, 0, 0.f};
     if (!p.rng) {
       w.st->u = p.u[row];
     } else if (!sr_row(p, row).greedy) {
@@ -316,12 +390,17 @@ __global__ __launch_bounds__(kSrThreads) void sample_extremes_kernel(SampleRowsP
   const SrLogits<T> lg(p, row);
   u64 top = 0;
   float low = INFINITY;
-  lg.template each<kSrThreads>(c, p.chunk, [&](float l, int i) {
-    const u64 k = sr_key(l, i);
-    top = k > top ? k : top;
-    if (l > -INFINITY) low = fminf(low, l);
+  float best = -INFINITY;                      // the thread's largest logit, and where it stood first
+  int where = 0;
+  lg.template each<kSrThreads>(c, p.chunk, [&](const float* l, int i) {
+#pragma unroll
+    for (int x = 0; x < SrLogits<T>::E; ++x) {
+      where = l[x] > best ? i + x : where;
+      best = fmaxf(best, l[x]);
+      low = fminf(low, l[x] > -INFINITY ? l[x] : INFINITY);
+    }
   });
-  top = wave_max_u64(top);
+  top = wave_max_u64(sr_key(best, where));
   low = wave_min(low);
   if ((t & 63) == 0) red[t >> 6] = top, lred[t >> 6] = low;
   __syncthreads();
@@ -335,7 +414,8 @@ __global__ __launch_bounds__(kSrThreads) void sample_extremes_kernel(SampleRowsP
   }
 }
 
-// 2. The histogram of a row with a cut; the others need none (the largest logit's row is done here).
+// 2. The histogram of a row with a cut. The others need none; rows of the largest logit, and those with no logit
+// to take, are done here.
 template <class T>
 __global__ __launch_bounds__(kSrThreads) void sample_histogram_kernel(SampleRowsParams p) {
   __shared__ u64 hm[kSrBuckets];
@@ -345,30 +425,35 @@ __global__ __launch_bounds__(kSrThreads) void sample_histogram_kernel(SampleRows
   const int row = blockIdx.x / p.chunks, c = blockIdx.x - row * p.chunks, t = threadIdx.x;
   const SrWork w = sr_work(p.work, row);
   const SrRow s = sr_row(p, row);
+  if (c > 0 && (s.greedy || !s.cut)) return;
   u64 top;
   float low;
-  sr_extremes(w, p.chunks, red, top, low);
+  SrExtremes(w, p.chunks).get(red, top, low);
   if (s.greedy || sr_none(top)) {
     if (c == 0 && t == 0) {
+      w.st->mode = SR_DONE;
       if (sr_none(top)) sr_put(p, row, -1, NAN);
       else sr_put(p, row, sr_index(top), 0.f);
     }
     return;
   }
-  if (!s.cut) {
-    if (c == 0 && t == 0) w.st->mode = SR_DRAW;
-    return;
-  }
+  if (!s.cut) return;
   for (int i = t; i < kSrBuckets; i += kSrThreads) hm[i] = 0, hc[i] = 0;
   __syncthreads();
   const SrScale sc(sr_logit(top), low, s.temperature, p.frac);
-  SrLogits<T>(p, row).template each<kSrThreads>(c, p.chunk, [&](float l, int) {
-    const u64 m = sc.mass(l);
-    if (m) {
-      const int b = sc.bucket(l);
-      atomicAdd(&hm[b], m);
-      atomicAdd(&hc[b], 1u);
-    }
+  constexpr int E = SrLogits<T>::E;
+  SrLogits<T>(p, row).template each<kSrThreads>(c, p.chunk, [&](const float* l, int) {
+    u64 m[E];
+    int b[E];
+#pragma unroll
+    for (int x = 0; x < E; ++x) b[x] = sc.bucket(l[x]);
+    sc.template masses<E>(l, m);
+#pragma unroll
+    for (int x = 0; x < E; ++x)
+      if (m[x]) {
+        atomicAdd(&hm[b[x]], m[x]);
+        atomicAdd(&hc[b[x]], 1u);
+      }
   });
   __syncthreads();
   for (int i = t; i < kSrBuckets; i += kSrThreads)
@@ -384,18 +469,15 @@ struct SrPlan {
   bool by_k;
   u64 base, total;
 };
-__device__ SrPlan sr_plan(const SrWork& w, const SrRow& s, u64* red) {
+constexpr int kSrOwn = kSrBuckets / kSrThreads;
+__device__ SrPlan sr_plan(const SrWork& w, const SrRow& s, const u64* m, const uint32_t* n, u64* red) {
   __shared__ int bk_s, bp_s;
   __shared__ u64 base_s[4], total_s[2];
   const int t = threadIdx.x;
-  constexpr int E = kSrBuckets / kSrThreads;
-  u64 m[E], msum = 0;
-  uint32_t n[E];
-  u64 nsum = 0;
+  constexpr int E = kSrOwn;
+  u64 msum = 0, nsum = 0;
 #pragma unroll
   for (int i = 0; i < E; ++i) {
-    m[i] = w.hmass[E * t + i];
-    n[i] = w.hcount[E * t + i];
     msum += m[i];
     nsum += n[i];
   }
@@ -444,11 +526,16 @@ __global__ __launch_bounds__(kSrThreads) void sample_gather_kernel(SampleRowsPar
   const int row = blockIdx.x / p.chunks, c = blockIdx.x - row * p.chunks, t = threadIdx.x;
   const SrWork w = sr_work(p.work, row);
   const SrRow s = sr_row(p, row);
+  if (s.greedy || !s.cut) return;
   u64 top;
   float low;
-  sr_extremes(w, p.chunks, red, top, low);
-  if (s.greedy || sr_none(top) || !s.cut) return;
-  const SrPlan q = sr_plan(w, s, red);
+  u64 m[kSrOwn];
+  uint32_t n[kSrOwn];
+#pragma unroll
+  for (int i = 0; i < kSrOwn; ++i) m[i] = w.hmass[kSrOwn * t + i], n[i] = w.hcount[kSrOwn * t + i];
+  SrExtremes(w, p.chunks).get(red, top, low);
+  if (sr_none(top)) return;
+  const SrPlan q = sr_plan(w, s, m, n, red);
   if (c == 0 && t == 0) {
     w.st->mode = q.mode;
     w.st->by_k = q.by_k;
@@ -457,39 +544,105 @@ __global__ __launch_bounds__(kSrThreads) void sample_gather_kernel(SampleRowsPar
   }
   if (q.mode != SR_FULL && q.mode != SR_EDGE) return;
   const SrScale sc(sr_logit(top), low, s.temperature, p.frac);
-  SrLogits<T>(p, row).template each<kSrThreads>(c, p.chunk, [&](float l, int i) {
-    if (!sc.mass(l)) return;
-    const int b = sc.bucket(l);
-    if (b < q.b0 || b > q.b1) return;
-    const int at = atomicAdd(&w.st->gathered, 1);
-    if (at < kSrGather) w.item[at] = sr_key(l, i);
+  // The block's tokens together in LDS, so that it counts them into the row's once; past the buffer one by one.
+  __shared__ u64 buf[kSrBlockGather];
+  __shared__ int found, at_s;
+  if (t == 0) found = 0;
+  __syncthreads();
+  const float least = sc.under(q.b1), most = q.b0 ? sc.over(q.b0) : INFINITY;
+  SrLogits<T>(p, row).template each<kSrThreads>(c, p.chunk, [&](const float* l, int i) {
+#pragma unroll
+    for (int x = 0; x < SrLogits<T>::E; ++x) {
+      if (l[x] < least || l[x] > most || !sc.mass(l[x])) continue;
+      const int b = sc.bucket(l[x]);
+      if (b < q.b0 || b > q.b1) continue;
+      const u64 key = sr_key(l[x], i + x);
+      const int at = atomicAdd(&found, 1);
+      if (at < kSrBlockGather) {
+        buf[at] = key;
+      } else {
+        const int g = atomicAdd(&w.st->gathered, 1);
+        if (g < kSrGather) w.item[g] = key;
+      }
+    }
   });
+  __syncthreads();
+  const int count = min(found, kSrBlockGather);
+  if (t == 0 && count) at_s = atomicAdd(&w.st->gathered, count);
+  __syncthreads();
+  for (int i = t; i < count; i += kSrThreads)
+    if (at_s + i < kSrGather) w.item[at_s + i] = buf[i];
 }
 
-// The (logit, index) at which the weights, added from the largest key down, reach `want`: eight bits a
-// round from the highest that differ. each(f) calls f(key, weight) over the thread's tokens.
+// The key at which the weights, added from the largest key down, reach `want`: BITS bits a round from the first
+// in which lo and hi differ, between which every key with a weight lies, until one token is left.
+// each(f) calls f(key, weight) over the thread's tokens.
+struct SrSelect {
+  u64 hist[kSrRowThreads], pick[2], key;
+  uint32_t count[kSrRowThreads];
+};
 template <class Each>
-__device__ u64 sr_select(Each each, u64 want, int bits, u64* hist, u64* red) {
-  __shared__ u64 pick_s[2];
+__device__ u64 sr_select(Each each, u64 want, u64 lo, u64 hi, SrSelect& x, u64* red) {
+  constexpr int BITS = __builtin_ctz(kSrRowThreads);  // a thread a bin
   const int t = threadIdx.x;
-  u64 prefix = 0;
-  for (int shift = bits - 8; shift >= 0; shift -= 8) {
-    if (t < 256) hist[t] = 0;
+  int bits = lo == hi ? 0 : 64 - __clzll(lo ^ hi);
+  u64 prefix = bits < 64 ? hi >> bits : 0;
+  while (bits > 0) {
+    const int shift = max(bits - BITS, 0), bins = 1 << (bits - shift), above = bits;
+    x.hist[t] = 0;
+    x.count[t] = 0;
     __syncthreads();
     each([&](u64 key, u64 wgt) {
-      if (wgt && (shift + 8 >= 64 ? 0 : key >> (shift + 8)) == prefix) atomicAdd(&hist[key >> shift & 255], wgt);
+      if (wgt && key >> above == prefix) {
+        const int b = (int)(key >> shift) & (bins - 1);
+        atomicAdd(&x.hist[b], wgt);
+        atomicAdd(&x.count[b], 1u);
+      }
     });
     __syncthreads();
-    // Thread i holds bin 255 - i.
-    const u64 v = t < 256 ? hist[255 - t] : 0;
+    // Thread i holds the i-th bin from above.
+    const int mine = bins - 1 - t;
+    const u64 v = mine >= 0 ? x.hist[mine] : 0;
     const u64 before = block_before_u64(v, red);
-    if (t < 256 && before < want && before + v >= want) pick_s[0] = 255 - t, pick_s[1] = before;
+    if (mine >= 0 && before < want && before + v >= want) x.pick[0] = mine, x.pick[1] = before;
     __syncthreads();
-    prefix = prefix << 8 | pick_s[0];
-    want -= pick_s[1];
+    const int b = (int)x.pick[0];
+    prefix = prefix << (bits - shift) | (u64)b;
+    want -= x.pick[1];
+    bits = shift;
+    if (shift > 0 && x.count[b] == 1) {
+      each([&](u64 key, u64 wgt) {
+        if (wgt && key >> shift == prefix) x.key = key;
+      });
+      __syncthreads();
+      prefix = x.key;
+      bits = 0;
+    }
     __syncthreads();
   }
   return prefix;
+}
+// The smallest and largest key with a weight, over the block.
+template <class Each>
+__device__ void sr_range(Each each, u64& lo, u64& hi, u64* red) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
+  u64 a = ~0ull, b = 0;
+  each([&](u64 key, u64 wgt) {
+    a = wgt && key < a ? key : a;
+    b = wgt && key > b ? key : b;
+  });
+  a = ~wave_max_u64(~a);
+  b = wave_max_u64(b);
+  __syncthreads();
+  if (lane == 0) red[w] = a, red[w + nw] = b;
+  __syncthreads();
+  for (int i = 0; i < nw; ++i) {
+    a = red[i] < a ? red[i] : a;
+    b = red[nw + i] > b ? red[nw + i] : b;
+  }
+  __syncthreads();
+  lo = a;
+  hi = b;
 }
 
 __device__ __forceinline__ void sr_store(const SampleRowsParams& p, int row, const SrScale& sc, float T, float l, int i,
@@ -498,98 +651,108 @@ __device__ __forceinline__ void sr_store(const SampleRowsParams& p, int row, con
   sr_put(p, row, i, p.logp ? (float)(d - log(ldexp((double)total, -sc.frac))) : 0.f);
 }
 
-// 4. A block a row: the cut, and the draw where every token that stayed was gathered.
+// 4. A block a row: the cut, and the draw where every token that stayed was gathered. Bound by the barriers and by
+// what every wave computes alike: 512 threads take 10.7 us for one row, 1024 12.7, 256 9.1; of 160 rows 20, 19, 26.
 template <class T>
 __global__ __launch_bounds__(kSrRowThreads) void sample_cut_kernel(SampleRowsParams p) {
   __shared__ u64 key_s[kSrGather], mass_s[kSrGather];
-  __shared__ u64 hist[256], red[16];
+  __shared__ SrSelect sel;
+  __shared__ u64 red[32];
   if (sr_gated(p)) return;
   const int row = blockIdx.x, t = threadIdx.x;
   const SrWork w = sr_work(p.work, row);
   const SrState st = *w.st;
-  if (st.mode == SR_DONE || st.mode == SR_DRAW) return;
+  SrExtremes ends(w, p.chunks);
+  constexpr int OWN = kSrGather / kSrRowThreads;
+  u64 item[OWN];                               // the thread's gathered tokens (some past the last one)
+#pragma unroll
+  for (int i = 0; i < OWN; ++i) item[i] = w.item[t + i * kSrRowThreads];
   const SrRow s = sr_row(p, row);
+  if (st.mode == SR_DONE || st.mode == SR_DRAW) return;
   u64 top;
   float low;
-  sr_extremes(w, p.chunks, red, top, low);
+  ends.get(red, top, low);
   const SrScale sc(sr_logit(top), low, s.temperature, p.frac);
-  constexpr int KB = 56;                       // bits of a key
   if (st.mode == SR_ROW) {
     const SrLogits<T> lg(p, row);
-    auto counts = [&](auto f) {
-      for (int c = 0; c < p.chunks; ++c)
-        lg.template each<kSrRowThreads>(c, p.chunk, [&](float l, int i) { f(sr_key(l, i), sc.mass(l) ? 1ull : 0ull); });
-    };
     auto masses = [&](auto f) {
-      for (int c = 0; c < p.chunks; ++c)
-        lg.template each<kSrRowThreads>(c, p.chunk, [&](float l, int i) { f(sr_key(l, i), sc.mass(l)); });
+      lg.template each<kSrRowThreads>(0, p.vocab, [&](const float* l, int i) {
+#pragma unroll
+        for (int x = 0; x < SrLogits<T>::E; ++x) f(sr_key(l[x], i + x), sc.mass(l[x]));
+      });
     };
+    auto counts = [&](auto f) { masses([&](u64 key, u64 wgt) { f(key, wgt ? 1ull : 0ull); }); };
+    const u64 lo = sr_key(low, kSrMaxVocab - 1);
     u64 cut = 0, total = st.total;
     if (st.by_k) {
-      cut = sr_select(counts, (u64)s.top_k, KB, hist, red);
+      cut = sr_select(counts, (u64)s.top_k, lo, top, sel, red);
       u64 m = 0;
       masses([&](u64 key, u64 wgt) { m += key >= cut ? wgt : 0; });
       total = block_sum_u64(m, red);
     }
     if (s.top_p < 1.f) {
-      const u64 c2 = sr_select(masses, sr_ceil(s.top_p, total), KB, hist, red);
+      const u64 c2 = sr_select(masses, sr_ceil(s.top_p, total), lo, top, sel, red);
       cut = c2 > cut ? c2 : cut;
     }
     if (t == 0) w.st->cut = cut, w.st->mode = SR_DRAW;
     return;
   }
   const int n = min(st.gathered, kSrGather);
-  for (int i = t; i < n; i += kSrRowThreads) {
-    const u64 k = w.item[i];
-    key_s[i] = k;
-    mass_s[i] = sc.mass(sr_logit(k));
-  }
+#pragma unroll
+  for (int i = 0; i < OWN; ++i)
+    if (t + i * kSrRowThreads < n) {
+      key_s[t + i * kSrRowThreads] = item[i];
+      mass_s[t + i * kSrRowThreads] = sc.mass(sr_logit(item[i]));
+    }
   __syncthreads();
-  auto masses = [&](auto f) {
+  u64 lo, hi;
+  sr_range([&](auto f) {
     for (int i = t; i < n; i += kSrRowThreads) f(key_s[i], mass_s[i]);
-  };
-  auto counts = [&](auto f) {
-    for (int i = t; i < n; i += kSrRowThreads) f(key_s[i], mass_s[i] ? 1ull : 0ull);
-  };
-  auto keep = [&](u64 cut) {                   // a thread's own tokens
-    for (int i = t; i < n; i += kSrRowThreads)
-      if (key_s[i] < cut) mass_s[i] = 0;
-  };
-  if (st.mode == SR_EDGE) {
-    const u64 cut = st.by_k ? sr_select(counts, (u64)s.top_k - st.base, KB, hist, red)
-                             : sr_select(masses, sr_ceil(s.top_p, st.total) - st.base, KB, hist, red);
-    if (t == 0) w.st->cut = cut, w.st->mode = SR_DRAW;
-    return;
-  }
+  }, lo, hi, red);
+  // The cut by count, the cut by mass, the draw, each a search.
+  const bool edge = st.mode == SR_EDGE;
   u64 total = st.total;
-  if (st.by_k) {
-    keep(sr_select(counts, (u64)s.top_k, KB, hist, red));
-    u64 m = 0;
-    masses([&](u64, u64 wgt) { m += wgt; });
-    total = block_sum_u64(m, red);
+#pragma unroll 1
+  for (int stage = 0; stage < 3; ++stage) {
+    if (stage == 0 ? !st.by_k : stage == 1 && (edge ? st.by_k : s.top_p >= 1.f)) continue;
+    if (!edge && (stage == 2 || (stage == 1 && st.by_k))) {
+      const u64 least = stage == 2 ? sc.floor_mass(s.min_p) : 0;
+      u64 m = 0;
+      for (int i = t; i < n; i += kSrRowThreads) {  // (a thread's own tokens)
+        if (mass_s[i] < least) mass_s[i] = 0;
+        m += mass_s[i];
+      }
+      total = block_sum_u64(m, red);
+    }
+    u64 want = stage == 0 ? (u64)s.top_k : stage == 1 ? sr_ceil(s.top_p, total) : sr_target(st.u, total) + 1;
+    if (edge) want -= st.base;
+    // The draw goes in index order: by the index part of the keys alone, which falls as the index rises.
+    const u64 part = stage == 2 ? (u64)(kSrMaxVocab - 1) : ~0ull;
+    if (stage == 2) lo = kSrMaxVocab - p.vocab, hi = kSrMaxVocab - 1;
+    const u64 key = sr_select([&](auto f) {
+      for (int i = t; i < n; i += kSrRowThreads) {
+        const u64 m = mass_s[i];
+        f(key_s[i] & part, stage == 0 && m ? 1 : m);
+      }
+    }, want, lo, hi, sel, red);
+    if (edge) {
+      if (t == 0) w.st->cut = key, w.st->mode = SR_DRAW;
+      return;
+    }
+    for (int i = t; i < n; i += kSrRowThreads) {
+      if (stage < 2 && key_s[i] < key) mass_s[i] = 0;
+      if (stage == 2 && mass_s[i] && (key_s[i] & part) == key)
+        sr_store(p, row, sc, s.temperature, sr_logit(key_s[i]), sr_index(key), total);
+    }
   }
-  if (s.top_p < 1.f) keep(sr_select(masses, sr_ceil(s.top_p, total), KB, hist, red));
-  const u64 least = sc.floor_mass(s.min_p);
-  u64 m = 0;
-  for (int i = t; i < n; i += kSrRowThreads) {
-    if (mass_s[i] < least) mass_s[i] = 0;
-    m += mass_s[i];
-  }
-  total = block_sum_u64(m, red);
-  // In index order: the index part of the keys alone, which falls as the index rises.
-  auto by_index = [&](auto f) {
-    for (int i = t; i < n; i += kSrRowThreads) f(key_s[i] & (kSrMaxVocab - 1), mass_s[i]);
-  };
-  const u64 pick = sr_select(by_index, sr_target(st.u, total) + 1, 24, hist, red);
-  for (int i = t; i < n; i += kSrRowThreads)
-    if (mass_s[i] && (key_s[i] & (kSrMaxVocab - 1)) == pick) sr_store(p, row, sc, s.temperature, sr_logit(key_s[i]), sr_index(pick), total);
   if (t == 0) w.st->mode = SR_DONE;
 }
 
-// 5. Each chunk's mass that stayed, for the rows not yet drawn.
+// 5. The mass that stayed in each part of a chunk, for the rows not yet drawn.
 template <class T>
 __global__ __launch_bounds__(kSrThreads) void sample_mass_kernel(SampleRowsParams p) {
   __shared__ u64 red[4];
+  __shared__ u64 part[kSrChunkParts][kSrThreads / 64];
   if (sr_gated(p)) return;
   const int row = blockIdx.x / p.chunks, c = blockIdx.x - row * p.chunks, t = threadIdx.x;
   const SrWork w = sr_work(p.work, row);
@@ -598,23 +761,44 @@ __global__ __launch_bounds__(kSrThreads) void sample_mass_kernel(SampleRowsParam
   const u64 cut = w.st->cut;
   u64 top;
   float low;
-  sr_extremes(w, p.chunks, red, top, low);
+  SrExtremes(w, p.chunks).get(red, top, low);
   const SrScale sc(sr_logit(top), low, s.temperature, p.frac);
   const u64 least = sc.floor_mass(s.min_p);
-  u64 sum = 0;
-  SrLogits<T>(p, row).template each<kSrThreads>(c, p.chunk, [&](float l, int i) {
-    const u64 m = sc.mass(l);
-    if (m >= least && sr_key(l, i) >= cut) sum += m;
+  // (logit, index) at least `cut`: above its logit, or that and no later than its index.
+  const float edge = cut ? sr_logit(cut) : -INFINITY;
+  const int last = cut ? sr_index(cut) : kSrMaxVocab;
+  const SrLogits<T> lg(p, row);
+  constexpr int E = SrLogits<T>::E;
+  u64 sum = 0;                                 // (the block's sums only at the end: no barriers between the parts)
+  int left = p.part, i = 0;
+  lg.template span<kSrThreads>(c * p.chunk, lg.end(c, p.chunk), [&](const float* l, int at) {
+    u64 m[E];
+    sc.template masses<E>(l, m);
+#pragma unroll
+    for (int x = 0; x < E; ++x)
+      sum += (m[x] >= least) & ((l[x] > edge) | ((l[x] == edge) & (at + x <= last))) ? m[x] : 0;
+  }, [&] {
+    left -= kSrThreads * E * SrLogits<T>::U;
+    if (left > 0) return;
+    sum = wave_upto_u64(sum);
+    if ((t & 63) == 63) part[i][t >> 6] = sum;
+    sum = 0;
+    left = p.part;
+    ++i;
   });
-  sum = block_sum_u64(sum, red);
-  if (t == 0) w.mass[c] = sum;
+  sum = wave_upto_u64(sum);                    // of a part that the row's end cuts short
+  if (i < p.parts && (t & 63) == 63) part[i][t >> 6] = sum;
+  for (++i; i < p.parts; ++i)
+    if ((t & 63) == 63) part[i][t >> 6] = 0;
+  __syncthreads();
+  if (t < p.parts) w.mass[c * p.parts + t] = part[t][0] + part[t][1] + part[t][2] + part[t][3];
 }
 
-// 6. The chunk that the draw falls into, and the token in it.
+// 6. The part that the draw falls into, and the token in it.
 template <class T>
 __global__ __launch_bounds__(kSrRowThreads) void sample_draw_kernel(SampleRowsParams p) {
   __shared__ u64 red[16], before_s;
-  __shared__ int chunk_s;
+  __shared__ int part_s;
   if (sr_gated(p)) return;
   const int row = blockIdx.x, t = threadIdx.x;
   const SrWork w = sr_work(p.work, row);
@@ -623,26 +807,31 @@ __global__ __launch_bounds__(kSrRowThreads) void sample_draw_kernel(SampleRowsPa
   const u64 cut = w.st->cut;
   u64 top;
   float low;
-  sr_extremes(w, p.chunks, red, top, low);
+  SrExtremes(w, p.chunks).get(red, top, low);
   const SrScale sc(sr_logit(top), low, s.temperature, p.frac);
   const u64 least = sc.floor_mass(s.min_p);
-  const u64 mc = t < p.chunks ? w.mass[t] : 0;
+  const u64 mc = t < p.chunks * p.parts ? w.mass[t] : 0;
   const u64 total = block_sum_u64(mc, red);
   u64 want = sr_target(w.st->u, total);
   const u64 bc = block_before_u64(mc, red);
-  if (bc <= want && want < bc + mc) chunk_s = t, before_s = bc;
+  if (bc <= want && want < bc + mc) part_s = t, before_s = bc;
   __syncthreads();
   want -= before_s;
   const SrLogits<T> lg(p, row);
-  const int c = chunk_s, i1 = lg.end(c, p.chunk);
-  for (int i0 = lg.begin(c, p.chunk); i0 < i1; i0 += 4 * kSrRowThreads) {
+  const int c = part_s / p.parts, first = c * p.chunk + (part_s - c * p.parts) * p.part;
+  const int i1 = min(lg.end(c, p.chunk), lg.end(0, first + p.part));
+  for (int i0 = first ? lg.head + first : 0; i0 < i1; i0 += 4 * kSrRowThreads) {
     u64 m[4], sum = 0;
     float l[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int i = i0 + 4 * t + k;
       l[k] = i < i1 ? lg.at(i) : -INFINITY;
-      m[k] = sc.mass(l[k]);
+    }
+    sc.template masses<4>(l, m);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = i0 + 4 * t + k;
       if (m[k] < least || sr_key(l[k], min(i, i1 - 1)) < cut) m[k] = 0;
       sum += m[k];
     }
@@ -716,8 +905,15 @@ int launch_sample_rows(const SampleRowsParams& params, hipStream_t s) {
   const char* why = sample_rows_refuses(p.n, p.vocab);
   TRX_CHECK(!why, TRX_E_INVALID, "sampling: %s", why);
   if (p.n == 0) return TRX_OK;
-  p.chunk = kSrChunk * std::max(1, cdiv(cdiv(p.vocab, kSrChunk), kSrChunksMax));
+  // About eight blocks a CU: many rows take long chunks (a chunk's histogram goes into the row's by atomics, as
+  // many as it has buckets), few rows short ones. 160 rows of 248320, with 1024, 2048, 4096 blocks in all: 212,
+  // 195, 187 us; 24 rows of 151936: 77, 78, 103. One row, with chunks of at least 1024, 2048, 4096: 45, 40, 40.
+  const int most = std::min(kSrChunksMax, std::max(1, cdiv(kSrBlocks, p.n)));
+  p.chunk = kSrChunk * cdiv(cdiv(p.vocab, kSrChunk), most);
   p.chunks = cdiv(p.vocab, p.chunk);
+  const int group = kSrThreads * SrLogits<float>::U * (p.half ? SrLogits<_Float16>::E : SrLogits<float>::E);
+  p.part = group * cdiv(cdiv(p.chunk, group), std::min(kSrChunkParts, kSrParts / p.chunks));
+  p.parts = cdiv(p.chunk, p.part);
   int bits = 0;
   while ((1 << bits) < p.vocab) ++bits;
   p.frac = std::min(51, 62 - bits);
