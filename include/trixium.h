@@ -223,7 +223,8 @@ int trx_gemv_packed_parts_f32(const uint8_t* packed, int kind, int M, int K, con
  * The ring holds the positions below pos that a query sees; slots that no visible position takes may
  * hold anything. Afterwards the new rows stand in their slots (of rows that share a slot, the last);
  * no other slot is written. An infinity or NaN in a key or value that a query does not see does not
- * reach its output; one in a value that it sees makes that element infinite or NaN. out, workspace and the ring overlap no other argument.
+ * reach its output; one in a value that it sees makes that element the same (inf and -inf: NaN). out,
+ * workspace and the ring overlap no other argument.
  * pos_dev != NULL: the first position is read from the device when the work runs (for captured
  * graphs) and `pos` is ignored; a position there that is negative or leaves int32 within n leaves out
  * and the ring as they are.

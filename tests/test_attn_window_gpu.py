@@ -395,3 +395,65 @@ def test_kv_ring_object():
     assert all(np.array_equal(a, b) for a, b in zip(ring.rows(), c.ring()))
     with pytest.raises(ValueError):
         ring.attend(q, k[:0], v)
+
+
+def _expect_by_head(c, q, k, v, gate):
+    """Case.expect for many heads and rows at once: a kv head's scores as one matrix."""
+    pos, n, rep, half = c.K.shape[0], q.shape[0], c.heads // c.kv, c.kind == F16
+    K = np.concatenate([c.K, k]).astype(np.float64)
+    V = np.concatenate([c.V, v]).astype(np.float64)
+    t, u = pos + np.arange(n)[:, None], np.arange(pos + n)[None]
+    seen = np.repeat((u <= t) & ((u < c.sinks) | (u > t - c.window)), rep, axis=0)
+    N = seen.sum(1)[:, None]
+    out = np.empty((n, c.heads, c.hd))
+    tol = np.empty_like(out)
+    for g in range(c.kv):
+        hs = slice(g * rep, (g + 1) * rep)
+        qd = q[:, hs].astype(np.float64).reshape(n * rep, c.hd)
+        s = np.where(seen, float(c.scale) * (qd @ K[:, g].T), -np.inf)
+        S = np.where(seen, float(c.scale) * (np.abs(qd) @ np.abs(K[:, g]).T), 0).max(1)[:, None]
+        p = np.exp(s - s.max(1)[:, None])
+        p /= p.sum(1)[:, None]
+        A, o = p @ np.abs(V[:, g]), p @ V[:, g]
+        e = A * (2 * (S * (2.0**-21 + c.hd * 2.0**-24) + 2.0**-21) + N * 2.0**-24 + 2.0**-22)
+        if half:
+            e += A * 2.0**-11 + N * 2.0**-32 * np.abs(V[:, g]).max()
+        sg = 1.0 / (1.0 + np.exp(-gate[:, hs].astype(np.float64).reshape(o.shape)))
+        o, e = o * sg, e * sg + np.abs(o) * 2.0**-21
+        if half:
+            e += np.abs(o) * 2.0**-11 + 2.0**-25
+        out[:, hs], tol[:, hs] = o.reshape(n, rep, c.hd), e.reshape(n, rep, c.hd)
+    return out, tol
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,heads,kv,hd,window,n", [
+    (F32, 32, 2, 64, 1000, 325), (F32, 24, 2, 64, 600, 695), (F16, 64, 4, 64, 1000, 140), (F16, 64, 32, 64, 1000, 177),
+    (F32, 64, 4, 128, 600, 140), (F32, 16, 4, 128, 2300, 180), (F32, 32, 32, 128, 100, 547), (F32, 16, 4, 128, 2300, 341),
+    (F16, 32, 32, 128, 1000, 177), (F16, 8, 8, 128, 1000, 547), (F16, 64, 32, 128, 1000, 177), (F16, 32, 32, 128, 1000, 140),
+    (F32, 64, 8, 256, 333, 140), (F32, 64, 4, 256, 333, 140), (F32, 32, 32, 256, 1000, 68), (F16, 64, 32, 256, 600, 54),
+    (F16, 32, 8, 256, 1000, 82), (F16, 64, 4, 256, 200, 140), (F16, 64, 32, 256, 1000, 33)])
+def test_many_columns(kind, heads, kv, hd, window, n):
+    """Calls with enough columns for the blocks of two and of four waves of them, with and without splits of
+    the keys, in each head size and type: the window across the ring's seam, slots that no position takes NaN.
+    One value seen by some rows alone is an infinity, in a tile that other rows see whole."""
+    c = Case(heads, kv, hd, slots=window + 90, pin=9, window=window, sinks=5, kind=kind, seed=11)
+    pos = window + 300
+    c.extend(pos)
+    c.K[7], c.V[7] = np.nan, np.nan                       # pinned, no sink, outside every window
+    q, k, v = c.rows(n)
+    gate = c.rng.standard_normal(q.shape).astype(DT[kind])
+    kc, vc = c.ring(np.nan)
+    late = 300 + window // 2                              # leaves the window after row window // 2
+    vc[:, c.slot(late), 3], vc[:, c.slot(late), hd - 1] = np.inf, -np.inf
+    out, _, _ = _call(c, q, k, v, kc, vc, gate)
+    out = out.reshape(n, heads, hd).astype(np.float64)
+    c.K[7], c.V[7] = 0, 0
+    want, tol = _expect_by_head(c, q, k, v, gate)
+    sees = np.zeros(out.shape, bool)
+    rows = pos + np.arange(n) - window < late
+    sees[rows, :, 3] = sees[rows, :, hd - 1] = True
+    assert (out[rows, :, 3] == np.inf).all() and (out[rows, :, hd - 1] == -np.inf).all()
+    err = np.abs(out - want)[~sees] / tol[~sees]
+    assert err.max() <= 1, float(err.max())
+    print(f"worst error {err.max():.3f} of the tolerance")

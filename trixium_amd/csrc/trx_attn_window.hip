@@ -377,9 +377,25 @@ struct AwWave {
       }
   }
 
+  // Whether a value was left out of a product, or a sum is infinite or NaN: an infinity's product with a
+  // probability's second plane, or with one that vanished, is not the infinity that the sum has to hold.
+  __device__ __forceinline__ bool stray() const {
+    float z = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) z = fmaf(o[dt][e], 0.f, z);
+    return __any(finite != ~0u || !(z == 0.f));
+  }
+  // Then: the sums without what is not finite, for add_seen. (NaN scores are in the sum of the probabilities.)
+  __device__ __forceinline__ void drop_strays() {
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[dt][e] = fabsf(o[dt][e]) < INFINITY ? o[dt][e] : 0.f;
+  }
   // The infinities and NaNs of the tile of keys from x0 on into the sums of the columns that see them, by a
   // product of their places with the keys seen: inf counts 1, -inf 64, NaN 4096, so 16 keys' counts do not mix.
-  // (Those that add took into a sum are put there once more, which changes nothing.)
   __device__ __forceinline__ void add_seen(const AwBlock& b, const AwRows<HD>& rows, int window, int t, int x0, int lane) {
     const int h = lane >> 5, j = lane & 31;
     f32x16_t none = {};
@@ -715,8 +731,10 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ * WK / 4) void attn_window_kernel(
       mask(st + 1);
     }
   }
-  if (__any(v.finite != ~0u))
+  if (v.stray()) {
+    v.drop_strays();
     for (int st = st0; st < st1; ++st) v.add_seen(b, rows, p.window, c.t, st * SR + wk * kAwKeys, lane);
+  }
   v.l += __shfl_xor(v.l, 32, 64);
   float mref = v.m == -INFINITY ? -INFINITY : v.m * v.cs;
   // Every wave's reads are done, and the K loaded past the last stage has arrived.
@@ -814,8 +832,10 @@ __global__ __launch_bounds__(256, 1) void attn_window_few_kernel(AttnWindowParam
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     v.add_masked(tr, ph, pl);
   }
-  if (__any(v.finite != ~0u))
+  if (v.stray()) {
+    v.drop_strays();
     for (int i = i0; i < i1; i += WK) v.add_seen(b, rows, p.window, c.t, i * kAwKeys, lane);
+  }
   v.l += __shfl_xor(v.l, 32, 64);
   float mref = v.m == -INFINITY ? -INFINITY : v.m * v.cs;
   __syncthreads();                                // every wave's reads are done
