@@ -28,6 +28,8 @@ struct AttnWindowParams {
   void* work;                  // attn_window_work_bytes
   // Set by the launcher.
   int rep, nsplit, cols;       // heads a kv head; splits of the keys; n * rep
+  unsigned long long rep_m;    // for the division by rep: a product with rep_m, shifted by rep_s
+  int rep_s;
 };
 
 // Why a geometry is not taken (null: it is).

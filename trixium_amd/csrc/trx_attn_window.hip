@@ -118,6 +118,16 @@ __device__ __forceinline__ uint32_t finite_h(uint32_t two) {
   return __builtin_bit_cast(uint32_t, x >> 15);
 }
 
+// The position's row of a column: column / rep by a product (columns below 2^28, rep_m = 2^rep_s / rep rounded up,
+// 2^rep_s at least 2^32 rep: exact).
+__device__ __forceinline__ int aw_row(const AttnWindowParams& p, int column) {
+  return (int)((unsigned long long)(unsigned)column * p.rep_m >> p.rep_s);
+}
+// The first of a split's share of `count` stages (count below 2^26, at most 64 splits).
+__device__ __forceinline__ int aw_share(int count, int split, int splits) {
+  return (int)((unsigned)count * (unsigned)split / (unsigned)splits);
+}
+
 // What the waves of a block know of their work: the call's first position and the block's keys, numbered
 // x in [0, N): position x below ns (the sinks), else x - ns + lo.
 struct AwBlock {
@@ -131,12 +141,12 @@ __device__ __forceinline__ AwBlock aw_block(const AttnWindowParams& p, int pos, 
   b.pos = pos;
   // A kv head's blocks stay on the XCDs of its number (blocks go round-robin over them): its K and V
   // are read into few L2s.
-  b.g = blockIdx.x % p.n_kv;
-  const int rest = blockIdx.x / p.n_kv;
-  b.sp = rest % p.nsplit;
-  b.c0 = rest / p.nsplit * columns;
-  b.t_first = pos + b.c0 / p.rep;
-  b.t_last = pos + min(b.c0 + columns - 1, p.cols - 1) / p.rep;
+  const unsigned cb = blockIdx.x / (unsigned)p.n_kv;
+  b.g = (int)(blockIdx.x - cb * p.n_kv);
+  b.sp = blockIdx.y;
+  b.c0 = (int)cb * columns;
+  b.t_first = pos + aw_row(p, b.c0);
+  b.t_last = pos + aw_row(p, min(b.c0 + columns - 1, p.cols - 1));
   b.ns = min(p.sinks, b.t_last + 1);
   b.lo = max(b.ns, b.t_first - p.window + 1);
   b.N = b.ns + (b.t_last + 1 - b.lo);
@@ -191,11 +201,11 @@ struct AwColumn {
 
   __device__ __forceinline__ AwColumn(const AttnWindowParams& p, const AwBlock& b, int first, int j) {
     const int last = p.cols - 1, col = min(first + j, last);
-    row = col / p.rep;
+    row = aw_row(p, col);
     head = b.g * p.rep + (col - row * p.rep);
     t = b.pos + row;
-    w_first = b.pos + min(first, last) / p.rep;
-    w_last = b.pos + min(first + 31, last) / p.rep;
+    w_first = b.pos + aw_row(p, min(first, last));
+    w_last = b.pos + aw_row(p, min(first + 31, last));
   }
 };
 
@@ -488,46 +498,48 @@ struct AwWave {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    const int d0 = 4 * (lane % L);
-    const size_t all = (size_t)p.nsplit * p.n_kv * p.cols;
-    int col = first + lane / L, row = col / p.rep, in = col - row * p.rep;  // the column's position and head
-    const int rows = CP / p.rep, heads = CP - rows * p.rep;
+    int col = first + lane / L, row = aw_row(p, col), in = col - row * p.rep;  // the column's position and head
+    const int rows = aw_row(p, CP), heads = CP - rows * p.rep;
 #pragma unroll 4
     for (int c = lane / L; c < 32; c += CP, col += CP) {
       if (col >= p.cols) break;
-      const float4 x = *(const float4*)(own + c * ST + d0);
+      const float4 x = *(const float4*)(own + c * ST + 4 * (lane % L));
       const float2 ml = *(const float2*)(own + c * ST + HD);
-      if (p.nsplit > 1) {
-        const size_t at = ((size_t)b.sp * p.n_kv + b.g) * p.cols + col;
-        *(float4*)((float*)p.work + at * HD + d0) = x;
-        if (d0 == 0) *((float2*)((float*)p.work + all * HD) + at) = ml;
-        continue;
-      }
-      const int head = b.g * p.rep + in;
-      const float inv = 1.0f / ml.y;
-      float v[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
-      const size_t orow = (size_t)row * p.out_stride + head * HD + d0;
-      const size_t grow = (size_t)row * p.gate_stride + (size_t)head * p.gate_head_stride + d0;
+      put(p, b, col, row, b.g * p.rep + in, 4 * (lane % L), x, ml);
       row += rows;
       in += heads;
       if (in >= p.rep) in -= p.rep, ++row;
-      if constexpr (HALF) {
-        if (p.gate) {
-          const half4_t gv = *(const half4_t*)((const _Float16*)p.gate + grow);
+    }
+  }
+  // Four dims of a column: its output, or its split's sums (the lane of dim 0 also the reference and the sum).
+  __device__ __forceinline__ static void put(const AttnWindowParams& p, const AwBlock& b, int col, int row, int head, int d0,
+                                             const float4& x, const float2& ml) {
+    if (p.nsplit > 1) {
+      const size_t all = (size_t)p.nsplit * p.n_kv * p.cols, at = ((size_t)b.sp * p.n_kv + b.g) * p.cols + col;
+      *(float4*)((float*)p.work + at * HD + d0) = x;
+      if (d0 == 0) *((float2*)((float*)p.work + all * HD) + at) = ml;
+      return;
+    }
+    const float inv = 1.0f / ml.y;
+    float v[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
+    const size_t orow = (size_t)row * p.out_stride + head * HD + d0;
+    const size_t grow = (size_t)row * p.gate_stride + (size_t)head * p.gate_head_stride + d0;
+    if constexpr (HALF) {
+      if (p.gate) {
+        const half4_t gv = *(const half4_t*)((const _Float16*)p.gate + grow);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) v[k] *= sigmoidf_((float)gv[k]);
-        }
-        *(half4_t*)((_Float16*)p.out + orow) = half4_t{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
-      } else {
-        if (p.gate) {
-          const float4 gv = *(const float4*)((const float*)p.gate + grow);
-          v[0] *= sigmoidf_(gv.x);
-          v[1] *= sigmoidf_(gv.y);
-          v[2] *= sigmoidf_(gv.z);
-          v[3] *= sigmoidf_(gv.w);
-        }
-        *(float4*)((float*)p.out + orow) = make_float4(v[0], v[1], v[2], v[3]);
+        for (int k = 0; k < 4; ++k) v[k] *= sigmoidf_((float)gv[k]);
       }
+      *(half4_t*)((_Float16*)p.out + orow) = half4_t{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+    } else {
+      if (p.gate) {
+        const float4 gv = *(const float4*)((const float*)p.gate + grow);
+        v[0] *= sigmoidf_(gv.x);
+        v[1] *= sigmoidf_(gv.y);
+        v[2] *= sigmoidf_(gv.z);
+        v[3] *= sigmoidf_(gv.w);
+      }
+      *(float4*)((float*)p.out + orow) = make_float4(v[0], v[1], v[2], v[3]);
     }
   }
 };
@@ -577,7 +589,7 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ * WK / 4) void attn_window_kernel(
   const AwColumn c(p, b, b.c0 + 32 * wq, j);
   const AwRows<HD> rows(p, b.g);
   const int stages = (b.N + SR - 1) / SR;
-  const int st0 = (int)((long long)stages * b.sp / p.nsplit), st1 = (int)((long long)stages * (b.sp + 1) / p.nsplit);
+  const int st0 = aw_share(stages, b.sp, p.nsplit), st1 = aw_share(stages, b.sp + 1, p.nsplit);
   const uint32_t ks = lds_address(smem), vs = ks + RING;
 
   // The block's queries come through LDS too, whole rows at a time and once for the WK waves: 16 bytes of each
@@ -587,7 +599,7 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ * WK / 4) void attn_window_kernel(
   {
     auto swizzle = [](int r) { return QP >= 16 ? r & 15 : r >> 1 & 7; };
     for (int i = w; i < (int)(QB / 1024); i += NW) {
-      const int r = (64 * i + lane) / QP, piece = lane % QP, col = min(b.c0 + r, p.cols - 1), row = col / p.rep;
+      const int r = (64 * i + lane) / QP, piece = lane % QP, col = min(b.c0 + r, p.cols - 1), row = aw_row(p, col);
       const size_t at = (size_t)row * p.q_stride + (b.g * p.rep + col - row * p.rep) * HD;
       load_lds16(ks + 1024 * i, (const char*)p.q + at * (HALF ? 2 : 4) + 16 * (piece ^ swizzle(r)));
     }
@@ -757,9 +769,11 @@ __global__ __launch_bounds__(256, 1) void attn_window_few_kernel(AttnWindowParam
   constexpr int WK = 4, SEG = HD / 8;
   constexpr int PP = kAwKeys * SEG / 64, RPP = 64 / SEG;  // a lane's 16-byte pieces of V; rows between them
   constexpr int VB = kAwKeys * Lds::ROW, QS = HD + 8;
-  constexpr size_t JOIN = (size_t)(WK - 1) * 64 * Wave::W * 4, STAGE = (size_t)WK * VB;
-  __shared__ __align__(1024) uint8_t smem[STAGE > JOIN ? STAGE : JOIN];
-  __shared__ __align__(16) _Float16 qs[HALF ? 1 : 2][32 * QS];
+  constexpr int QROW = HD * (HALF ? 2 : 4), QP = QROW / 16;  // bytes of a query; its 16-byte pieces
+  constexpr size_t STAGE = (size_t)WK * VB, PLANES = (HALF ? 1 : 2) * 32 * QS * 2, JOIN = (size_t)WK * 64 * Wave::W * 4;
+  static_assert(32 * QROW <= STAGE, "the queries as they come fit where the V rows will be");
+  __shared__ __align__(1024) uint8_t smem[STAGE + PLANES > JOIN ? STAGE + PLANES : JOIN];
+  _Float16* const qs = (_Float16*)(smem + STAGE);
 
   int pos;
   if (!aw_pos(p, pos)) return;
@@ -769,7 +783,8 @@ __global__ __launch_bounds__(256, 1) void attn_window_few_kernel(AttnWindowParam
   const AwColumn c(p, b, b.c0, j);
   const AwRows<HD> rows(p, b.g);
   const int tiles = (b.N + kAwKeys - 1) / kAwKeys;
-  const int i0 = (int)((long long)tiles * b.sp / p.nsplit) + wk, i1 = (int)((long long)tiles * (b.sp + 1) / p.nsplit);
+  const int i0 = aw_share(tiles, b.sp, p.nsplit) + wk, i1 = aw_share(tiles, b.sp + 1, p.nsplit);
+  const int columns = min(32, p.cols - b.c0), mine = min(j, columns - 1);
   uint8_t* const vs = smem + wk * VB;
   const int srow = lane / SEG, piece = lane % SEG;
   const uint32_t tr = aw_tr<HD>(lds_address(vs), lane);
@@ -792,31 +807,42 @@ __global__ __launch_bounds__(256, 1) void attn_window_few_kernel(AttnWindowParam
       vr[k] = *(const u32x4_t*)(rows.vc + (a & ~1ll) + (rows.vd & -(a & 1)) + 16 * piece);
     }
   };
+  // The queries there are, whole rows at a time, into LDS, beside the first rows; then their planes.
+  auto swizzle = [](int r) { return QP >= 16 ? r & 15 : r >> 1 & 7; };
+  for (int i = wk; 1024 * i < columns * QROW; i += WK) {
+    const int r = min((64 * i + lane) / QP, columns - 1), row = aw_row(p, b.c0 + r);
+    const size_t at = (size_t)row * p.q_stride + (b.g * p.rep + b.c0 + r - row * p.rep) * HD;
+    load_lds16(lds_address(smem) + 1024 * i, (const char*)p.q + at * (HALF ? 2 : 4) + 16 * (lane % QP ^ swizzle((64 * i + lane) / QP)));
+  }
   if (i0 < i1) {
     load_k(i0);
     load_v(i0);
   }
+  wait_loads_and_block<0>();
   Wave v;
   {
     AwQuery<HD, HALF> q;
-    const char* qr = (const char*)p.q + ((size_t)c.row * p.q_stride + c.head * HD) * (HALF ? 2 : 4);
-    v.init(q.take(p.scale, h, [&](int i) { return *(const u32x4_t*)(qr + 16 * i); }));
-    if (wk == 0) {
+    const uint32_t at = lds_address(smem) + mine * QROW;
+    v.init(q.take(p.scale, h, [&](int i) { return __builtin_bit_cast(u32x4_t, lds_half8(at + 16 * (i ^ swizzle(mine)))); }));
 #pragma unroll
-      for (int k = 0; k < Wave::NC; ++k) {
-        *(half8_t*)(qs[0] + j * QS + 16 * k + 8 * h) = q.hi[k];
-        if constexpr (!HALF) *(half8_t*)(qs[HALF ? 0 : 1] + j * QS + 16 * k + 8 * h) = q.lo[k];
+    for (int k = 0; k < Wave::NC; ++k)
+      if (k % WK == wk) {
+        *(half8_t*)(qs + j * QS + 16 * k + 8 * h) = q.hi[k];
+        if constexpr (!HALF) *(half8_t*)(qs + 32 * QS + j * QS + 16 * k + 8 * h) = q.lo[k];
       }
-    }
   }
   __syncthreads();
-  const _Float16* const qr = qs[0] + j * QS + 8 * h;
+  const _Float16* const qr = qs + j * QS + 8 * h;
   for (int i = i0; i < i1; i += WK) {
     f32x16_t s = Wave::scores([&](int k) { return kf[k]; }, [&](int k) { return *(const half8_t*)(qr + 16 * k); },
                               [&](int k) { return *(const half8_t*)(qr + 32 * QS + 16 * k); });
     const bool more = i + WK < i1;
     if (more) load_k(i + WK);
-    v.mask(b, p.window, c.t, i * kAwKeys, h, s);
+    // Whether every column of the wave sees every key (a second form of the products is more than the registers
+    // hold with 256 dims).
+    const int x0 = i * kAwKeys, u0 = x0 - b.ns + b.lo;
+    const bool whole = HD < 256 && x0 >= b.ns && u0 > c.w_last - p.window && u0 + kAwKeys - 1 <= c.w_first;
+    if (!whole) v.mask(b, p.window, c.t, x0, h, s);
     v.raise(s);
     half8_t ph[2], pl[2];
     v.probabilities(s, ph, pl);
@@ -830,7 +856,8 @@ __global__ __launch_bounds__(256, 1) void attn_window_few_kernel(AttnWindowParam
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    v.add_masked(tr, ph, pl);
+    if (whole) v.add(tr, ph, pl);
+    else v.add_masked(tr, ph, pl);
   }
   if (v.stray()) {
     v.drop_strays();
@@ -838,9 +865,46 @@ __global__ __launch_bounds__(256, 1) void attn_window_few_kernel(AttnWindowParam
   }
   v.l += __shfl_xor(v.l, 32, 64);
   float mref = v.m == -INFINITY ? -INFINITY : v.m * v.cs;
+  // The four waves' sums joined, each wave's share of the dims.
   __syncthreads();                                // every wave's reads are done
-  if (!v.template join<1, WK>((float*)smem, 0, wk, lane, mref)) return;
-  v.finish(p, b, b.c0, lane, mref, (float*)smem);
+  float* const jb = (float*)smem + lane;
+  if (j < columns) {
+    float* const to = jb + (size_t)wk * Wave::W * 64;
+#pragma unroll
+    for (int dt = 0; dt < Wave::NDT; ++dt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) to[(dt * 16 + e) * 64] = v.o[dt][e];
+    to[(Wave::W - 2) * 64] = mref;
+    to[(Wave::W - 1) * 64] = v.l;
+  }
+  __syncthreads();
+  if (j >= columns) return;
+  float M = -INFINITY, l = 0.f, f[WK];
+#pragma unroll
+  for (int i = 0; i < WK; ++i) M = fmaxf(M, f[i] = jb[((size_t)i * Wave::W + Wave::W - 2) * 64]);
+#pragma unroll
+  for (int i = 0; i < WK; ++i) {
+    // A wave that saw no key leaves nothing (its sums are zero).
+    f[i] = f[i] == -INFINITY ? 0.f : f[i] == M ? 1.f : __builtin_amdgcn_exp2f(f[i] - M);
+    l += jb[((size_t)i * Wave::W + Wave::W - 1) * 64] * f[i];
+  }
+  constexpr int OWN = Wave::NDT >= WK ? Wave::NDT / WK : 1;
+#pragma unroll
+  for (int d = 0; d < OWN; ++d) {
+    const int dt = wk * OWN + d;
+    if (dt >= Wave::NDT) return;
+    float x[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < WK; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[e] += jb[((size_t)i * Wave::W + dt * 16 + e) * 64] * f[i];
+#pragma unroll
+    for (int a4 = 0; a4 < 4; ++a4)
+      Wave::put(p, b, b.c0 + j, c.row, c.head, dt * 32 + 8 * a4 + 4 * h,
+                make_float4(x[4 * a4], x[4 * a4 + 1], x[4 * a4 + 2], x[4 * a4 + 3]), make_float2(M, l));
+  }
 }
 
 // After the attention: the splits of each (position, head) joined (a wave each, blocks of four), and
@@ -852,9 +916,9 @@ __global__ __launch_bounds__(256) void attn_window_finish(AttnWindowParams p, in
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   if ((int)blockIdx.x < join_blocks) {
     constexpr int E = HD / 64;                     // dims a lane: E lane .. + E - 1
-    const long long id = (long long)blockIdx.x * 4 + w;
-    if (id >= (long long)p.n * p.n_head) return;
-    const int row = (int)(id / p.n_head), head = (int)(id - (long long)row * p.n_head), g = head / p.rep;
+    const unsigned id = blockIdx.x * 4 + w;         // below 2^28 + 4
+    if (id >= (unsigned)(p.n * p.n_head)) return;
+    const int row = (int)(id / (unsigned)p.n_head), head = (int)id - row * p.n_head, g = aw_row(p, head);
     const int col = row * p.rep + head - g * p.rep;
     const size_t all = (size_t)p.nsplit * p.n_kv * p.cols, step = (size_t)p.n_kv * p.cols;
     const size_t at = (size_t)g * p.cols + col;
@@ -908,7 +972,8 @@ __global__ __launch_bounds__(256) void attn_window_finish(AttnWindowParams p, in
   const long long id = (long long)(blockIdx.x - join_blocks) * 256 + threadIdx.x;
   const long long pieces = (long long)p.n * p.n_kv * SEG;
   if (id >= pieces) return;
-  const int sd = (int)(id % SEG) * 8, g = (int)(id / SEG % p.n_kv), r = (int)(id / SEG / p.n_kv), u = pos + r;
+  const unsigned at = (unsigned)(id / SEG);        // below 2^28
+  const int sd = (int)(id % SEG) * 8, r = (int)(at / (unsigned)p.n_kv), g = (int)at - r * p.n_kv, u = pos + r;
   if (u >= p.pin && p.n - r > R) return;
   const int slot = u < p.pin ? u : p.pin + (int)((unsigned)(u - p.pin) % (unsigned)R);
   const size_t to = ((size_t)g * p.slots + slot) * HD + sd, from = (size_t)r * p.kv_stride + (size_t)g * HD + sd;
@@ -994,7 +1059,7 @@ size_t attn_window_work_bytes(const AttnWindowParams& p) {
 template <int HD, bool HALF>
 static int aw_launch(const AttnWindowParams& p, int wq, hipStream_t s) {
   constexpr int WT = HD == 256 ? 4 : 8;              // waves of the kernel for many columns
-  const dim3 grid(cdiv(p.cols, 32 * wq) * p.n_kv * p.nsplit);
+  const dim3 grid(cdiv(p.cols, 32 * wq) * p.n_kv, p.nsplit);
   if (wq == 1) hipLaunchKernelGGL((attn_window_few_kernel<HD, HALF>), grid, dim3(256), 0, s, p);
   else if (wq == 2) hipLaunchKernelGGL((attn_window_kernel<HD, HALF, 2, WT / 2, HD == 64 ? 2 : 1>), grid, dim3(64 * WT), 0, s, p);
   else hipLaunchKernelGGL((attn_window_kernel<HD, HALF, 4, WT / 4, 2>), grid, dim3(64 * WT), 0, s, p);
@@ -1013,6 +1078,9 @@ int launch_attn_window(const AttnWindowParams& params, hipStream_t s) {
   if (p.n == 0) return TRX_OK;
   p.rep = p.n_head / p.n_kv;
   p.cols = p.n * p.rep;
+  p.rep_s = 32;
+  while (1 << (p.rep_s - 32) < p.rep) ++p.rep_s;
+  p.rep_m = ((1ull << p.rep_s) + p.rep - 1) / p.rep;
   // The workspace holds the splits of a full window; a ring that is still filling takes no more.
   AwPlan plan = aw_plan(p, LLONG_MAX / 2, kAwMaxSplits);
   if (!p.pos_dev && p.pos < (long long)p.sinks + p.window) plan = aw_plan(p, p.pos, plan.nsplit);
