@@ -310,18 +310,20 @@ __device__ __forceinline__ u64 block_sum_u64(u64 v, u64* red) {
     if (i < nw) t += red[i];
   return t;
 }
-// Sum of the values of the threads before this one.
-__device__ __forceinline__ u64 block_before_u64(u64 v, u64* red) {
+// Sum of the values of the threads before this one, and of all.
+__device__ __forceinline__ u64 block_before_u64(u64 v, u64* red, u64& all) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
   const u64 x = wave_upto_u64(v);
   __syncthreads();
   if (lane == 63) red[w] = x;
   __syncthreads();
   u64 t = 0;
+  all = 0;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const u64 r = i < nw ? red[i] : 0;
     t += i < w ? r : 0;
+    all += r;
   }
   return t + x - v;
 }
@@ -472,7 +474,7 @@ struct SrPlan {
 constexpr int kSrOwn = kSrBuckets / kSrThreads;
 __device__ SrPlan sr_plan(const SrWork& w, const SrRow& s, const u64* m, const uint32_t* n, u64* red) {
   __shared__ int bk_s, bp_s;
-  __shared__ u64 base_s[4], total_s[2];
+  __shared__ u64 base_s[4];
   const int t = threadIdx.x;
   constexpr int E = kSrOwn;
   u64 msum = 0, nsum = 0;
@@ -481,11 +483,10 @@ __device__ SrPlan sr_plan(const SrWork& w, const SrRow& s, const u64* m, const u
     msum += m[i];
     nsum += n[i];
   }
-  u64 mb = block_before_u64(msum, red), nb = block_before_u64(nsum, red);
-  if (t == kSrThreads - 1) total_s[0] = mb + msum, total_s[1] = nb + nsum;
+  u64 total, live;
+  u64 mb = block_before_u64(msum, red, total), nb = block_before_u64(nsum, red, live);
   if (t == 0) bk_s = bp_s = -1;
   __syncthreads();
-  const u64 total = total_s[0], live = total_s[1];
   const bool by_k = s.top_k > 0 && (u64)s.top_k < live, by_p = s.top_p < 1.f;
   const u64 want_p = by_p ? sr_ceil(s.top_p, total) : 0;
 #pragma unroll
@@ -551,6 +552,10 @@ __global__ __launch_bounds__(kSrThreads) void sample_gather_kernel(SampleRowsPar
   __syncthreads();
   const float least = sc.under(q.b1), most = q.b0 ? sc.over(q.b0) : INFINITY;
   SrLogits<T>(p, row).template each<kSrThreads>(c, p.chunk, [&](const float* l, int i) {
+    bool some = false;
+#pragma unroll
+    for (int x = 0; x < SrLogits<T>::E; ++x) some |= (l[x] >= least) & (l[x] <= most);
+    if (!some) return;
 #pragma unroll
     for (int x = 0; x < SrLogits<T>::E; ++x) {
       if (l[x] < least || l[x] > most || !sc.mass(l[x])) continue;
@@ -603,7 +608,8 @@ __device__ u64 sr_select(Each each, u64 want, u64 lo, u64 hi, SrSelect& x, u64* 
     // Thread i holds the i-th bin from above.
     const int mine = bins - 1 - t;
     const u64 v = mine >= 0 ? x.hist[mine] : 0;
-    const u64 before = block_before_u64(v, red);
+    u64 all;
+    const u64 before = block_before_u64(v, red, all);
     if (mine >= 0 && before < want && before + v >= want) x.pick[0] = mine, x.pick[1] = before;
     __syncthreads();
     const int b = (int)x.pick[0];
@@ -811,9 +817,9 @@ __global__ __launch_bounds__(kSrRowThreads) void sample_draw_kernel(SampleRowsPa
   const SrScale sc(sr_logit(top), low, s.temperature, p.frac);
   const u64 least = sc.floor_mass(s.min_p);
   const u64 mc = t < p.chunks * p.parts ? w.mass[t] : 0;
-  const u64 total = block_sum_u64(mc, red);
+  u64 total;
+  const u64 bc = block_before_u64(mc, red, total);
   u64 want = sr_target(w.st->u, total);
-  const u64 bc = block_before_u64(mc, red);
   if (bc <= want && want < bc + mc) part_s = t, before_s = bc;
   __syncthreads();
   want -= before_s;
@@ -835,13 +841,12 @@ __global__ __launch_bounds__(kSrRowThreads) void sample_draw_kernel(SampleRowsPa
       if (m[k] < least || sr_key(l[k], min(i, i1 - 1)) < cut) m[k] = 0;
       sum += m[k];
     }
-    u64 b = block_before_u64(sum, red);
+    u64 all, b = block_before_u64(sum, red, all);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       if (b <= want && want < b + m[k]) sr_store(p, row, sc, s.temperature, l[k], i0 + 4 * t + k, total);
       b += m[k];
     }
-    const u64 all = block_sum_u64(sum, red);
     if (want < all) return;
     want -= all;
   }
