@@ -457,3 +457,24 @@ def test_many_columns(kind, heads, kv, hd, window, n):
     err = np.abs(out - want)[~sees] / tol[~sees]
     assert err.max() <= 1, float(err.max())
     print(f"worst error {err.max():.3f} of the tolerance")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,heads,kv,hd,n", [(F32, 4, 2, 64, 1), (F32, 4, 2, 64, 37), (F16, 6, 1, 256, 5),
+                                                (F16, 64, 4, 64, 140), (F32, 64, 4, 128, 140)])
+def test_positions_up_to_the_largest(kind, heads, kv, hd, n):
+    """Without pinned rows the outputs depend on the position's place in the ring alone: the last n positions
+    that int32 holds give the bits of earlier ones at the same place; one more is refused."""
+    R = 900
+    c = Case(heads, kv, hd, slots=R, pin=0, window=800, sinks=0, kind=kind, seed=12)
+    q, k, v = c.rows(n)
+    _, kc, vc = c.rows(R)
+    kc, vc = (np.ascontiguousarray(a.transpose(1, 0, 2)) for a in (kc, vc))
+    top = 2**31 - 1 - n
+    low = top - (top - 5000) // R * R
+    a, b = (_call(c, q, k, v, kc, vc, pos=p) for p in (top, low))
+    assert np.isfinite(a[0]).all()
+    for x, y in zip(a, b):
+        assert np.array_equal(x.view(np.uint8), y.view(np.uint8))
+    with pytest.raises(_lib.TrxError):
+        _call(c, q, k, v, kc, vc, pos=top + 1)

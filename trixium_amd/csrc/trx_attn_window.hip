@@ -183,8 +183,9 @@ struct AwRows {
   // How many runs of `count` keys from key x0 on lie evenly spaced (uniform); with one at least, the first
   // one's distance and the step in bytes.
   __device__ __forceinline__ int flat(const AwBlock& b, int x0, int count, long long& at, bool& own, uint32_t& step) const {
+    if (x0 < b.ns || x0 >= b.N) return 0;
     const int u0 = x0 - b.ns + b.lo;
-    if (x0 < b.ns || u0 < pin) return 0;
+    if (u0 < pin) return 0;
     int ro = b.roff + (u0 - b.ub);
     ro = ro >= b.R ? ro - b.R : ro;
     own = u0 >= b.pos;
@@ -298,10 +299,11 @@ struct AwWave {
   // -inf at the keys that the column does not see; the bits of the others.
   __device__ __forceinline__ uint32_t mask(const AwBlock& b, int window, int t, int x0, int h, f32x16_t& s) const {
     uint32_t vis = 0;
+    const int last = t - b.lo + b.ns;              // the number of the column's own position: key x is last - x before
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      const int x = x0 + 8 * (e >> 2) + 4 * h + (e & 3), u = x - b.ns + b.lo;
-      const bool ok = (x < b.ns & x <= t) | (x >= b.ns & u <= t & u > t - window);
+      const int x = x0 + 8 * (e >> 2) + 4 * h + (e & 3);
+      const bool ok = x < b.ns ? x <= t : (unsigned)(last - x) < (unsigned)window;
       s[e] = ok ? s[e] : -INFINITY;
       vis |= (uint32_t)ok << e;
     }
@@ -841,7 +843,7 @@ __global__ __launch_bounds__(256, 1) void attn_window_few_kernel(AttnWindowParam
     // Whether every column of the wave sees every key (a second form of the products is more than the registers
     // hold with 256 dims).
     const int x0 = i * kAwKeys, u0 = x0 - b.ns + b.lo;
-    const bool whole = HD < 256 && x0 >= b.ns && u0 > c.w_last - p.window && u0 + kAwKeys - 1 <= c.w_first;
+    const bool whole = HD < 256 && x0 >= b.ns && u0 > c.w_last - p.window && u0 <= c.w_first - (kAwKeys - 1);
     if (!whole) v.mask(b, p.window, c.t, x0, h, s);
     v.raise(s);
     half8_t ph[2], pl[2];
