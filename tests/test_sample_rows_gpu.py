@@ -278,3 +278,22 @@ def test_captured_graph_reads_new_settings_and_numbers():
         assert np.array_equal(sample(lg, us, **kw)[0], got)            # eager work between the replays
     _lib.call("trx_graph_destroy", ex)
     _lib.call("trx_stream_destroy", s)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("vocab,n", [(20011, 600), (9001, 2100), (33000, 129), (2**21 + 5, 2)])
+def test_rows_cut_into_long_chunks(vocab, n, dtype):
+    """Many rows and the longest ones take chunks of several rounds and parts: some rows of each setting
+    against the definition, and every row's token again when the row is drawn alone with others."""
+    rng = np.random.default_rng(vocab)
+    lg = (4.0 * rng.standard_normal((n, vocab), dtype=np.float32)).astype(dtype)
+    u = rng.random(n).astype(np.float32)
+    kw = _mixed(n)
+    tok, lp = sample(lg, u, **kw)
+    some = rng.permutation(n)[:15]
+    check(lg[some], u[some], **{k: v[some] for k, v in kw.items()})
+    again, lp2 = sample(lg[some], u[some], **{k: v[some] for k, v in kw.items()})
+    assert np.array_equal(tok[some], again) and np.array_equal(lp[some], lp2)
+    for r in some[:4]:
+        assert oracle(lg[r], u[r], *(kw[k][r] for k in ROW.names))[0] == tok[r]
