@@ -26,6 +26,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 #include <limits.h>
 
 namespace trx {
@@ -926,25 +927,39 @@ __global__ __launch_bounds__(256) void attn_window_finish(AttnWindowParams p, in
     const size_t at = (size_t)g * p.cols + col;
     const float2* ml = (const float2*)((const float*)p.work + all * HD) + at;
     const float* po = (const float*)p.work + at * HD + E * lane;
-    float M = -INFINITY;
-    for (int s = lane; s < p.nsplit; s += 64) M = fmaxf(M, ml[s * step].x);
-    M = wave_max(M);
-    float l = 0.f, o[E];
+    const size_t gi = (size_t)row * p.gate_stride + (size_t)head * p.gate_head_stride + E * lane;
+    const size_t oi = (size_t)row * p.out_stride + (size_t)head * HD + E * lane;
+    typedef typename std::conditional<HALF, _Float16, float>::type io_t;
+    io_t gate[E], out[E];
+    if (p.gate) __builtin_memcpy(gate, (const io_t*)p.gate + gi, sizeof gate);
+    float M = -INFINITY, l = 0.f, o[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) o[i] = 0.f;
-    // Eight splits' loads at a time in flight.
+    // Eight splits' loads at a time in flight (the gate's with them), a running reference over the eights.
     for (int s0 = 0; s0 < p.nsplit; s0 += 8) {
       float2 a[8];
       float x[8][E];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const int s = min(s0 + k, p.nsplit - 1);
-        a[k] = ml[s * step];
-        __builtin_memcpy(x[k], po + s * step * HD, 4 * E);
+        a[k] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[k][i] = 0.f;
+        if (s0 + k < p.nsplit) {
+          a[k] = ml[(s0 + k) * step];
+          __builtin_memcpy(x[k], po + (s0 + k) * step * HD, 4 * E);
+        }
       }
+      float top = M;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) top = fmaxf(top, a[k].x);
+      const float keep = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - top);
+      M = top;
+      l *= keep;
+#pragma unroll
+      for (int i = 0; i < E; ++i) o[i] *= keep;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float f = s0 + k >= p.nsplit || a[k].x == -INFINITY ? 0.f : a[k].x == M ? 1.f : __builtin_amdgcn_exp2f(a[k].x - M);
+        const float f = a[k].x == -INFINITY ? 0.f : a[k].x == M ? 1.f : __builtin_amdgcn_exp2f(a[k].x - M);
         l += a[k].y * f;
 #pragma unroll
         for (int i = 0; i < E; ++i) o[i] += x[k][i] * f;
@@ -953,18 +968,10 @@ __global__ __launch_bounds__(256) void attn_window_finish(AttnWindowParams p, in
     const float inv = 1.0f / l;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      const int d = E * lane + i;
-      float v = o[i] * inv;
-      const size_t gi = (size_t)row * p.gate_stride + (size_t)head * p.gate_head_stride + d;
-      const size_t oi = (size_t)row * p.out_stride + (size_t)head * HD + d;
-      if constexpr (HALF) {
-        if (p.gate) v *= sigmoidf_((float)((const _Float16*)p.gate)[gi]);
-        ((_Float16*)p.out)[oi] = (_Float16)v;
-      } else {
-        if (p.gate) v *= sigmoidf_(((const float*)p.gate)[gi]);
-        ((float*)p.out)[oi] = v;
-      }
+      const float v = o[i] * inv;
+      out[i] = (io_t)(p.gate ? v * sigmoidf_((float)gate[i]) : v);
     }
+    __builtin_memcpy((io_t*)p.out + oi, out, sizeof out);
     return;
   }
   // Rows pos .. pos + n - 1, 16 bytes of K and V a thread. A ring row that a later row of the call
