@@ -20,7 +20,7 @@
 // What bounds it: many rows, reading them (the largest logits, the histogram, the gather; for a row drawn from more
 // than was gathered, the masses) and the 64-bit exponentials; a single row, six launches that wait for each other.
 // us per launch, 160 rows of 248320 fp32 logits (159 MB) with top_p: 28 (5.7 TB/s), 61 (without the
-// exponentials 42), 41, the cuts 20, masses 20, draws 10; one row of 151936: 4, 7, 7, 11, 1 to 4, 1.
+// exponentials 42), 42, the cuts 20, masses 20, draws 9; one row of 151936: 4, 7, 7, 4, 2, 1.
 
 #include "trx_sample.h"
 
@@ -272,15 +272,6 @@ struct SrLogits {
   }
 };
 
-__device__ __forceinline__ u64 wave_max_u64(u64 v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    const u64 x = __shfl_xor(v, o, 64);
-    v = x > v ? x : v;
-  }
-  return v;
-}
-__device__ __forceinline__ float wave_min(float v) { return -wave_max(-v); }
 // The sum of this lane's value and those of the lanes before it: rows of 16 by shifts, then the rows' ends.
 template <int CTRL, int ROWS>
 __device__ __forceinline__ u64 dpp_u64(u64 v) {
@@ -296,6 +287,35 @@ __device__ __forceinline__ u64 wave_upto_u64(u64 v) {
   v += dpp_u64<0x142, 0xA>(v);                 // row_bcast 15 into rows 1 and 3
   v += dpp_u64<0x143, 0xC>(v);                 // row_bcast 31 into rows 2 and 3
   return v;
+}
+__device__ __forceinline__ u64 wave_lane_u64(u64 v, int lane) {
+  return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+}
+__device__ __forceinline__ u64 wave_sum_u64(u64 v) { return wave_lane_u64(wave_upto_u64(v), 63); }
+// The largest value of the wave (every lane gets it), the same way.
+__device__ __forceinline__ u64 wave_max_u64(u64 v) {
+  const auto up = [&](u64 x) __attribute__((always_inline)) { v = x > v ? x : v; };
+  up(dpp_u64<0x111, 0xF>(v));
+  up(dpp_u64<0x112, 0xF>(v));
+  up(dpp_u64<0x114, 0xF>(v));
+  up(dpp_u64<0x118, 0xF>(v));
+  up(dpp_u64<0x142, 0xA>(v));
+  up(dpp_u64<0x143, 0xC>(v));
+  return wave_lane_u64(v, 63);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_min(float v) {
+  return fminf(v, __int_as_float(__builtin_amdgcn_update_dpp(0x7F800000, __float_as_int(v), CTRL, ROWS, 0xF, false)));
+}
+__device__ __forceinline__ float wave_min(float v) {
+  v = dpp_min<0x111, 0xF>(v);
+  v = dpp_min<0x112, 0xF>(v);
+  v = dpp_min<0x114, 0xF>(v);
+  v = dpp_min<0x118, 0xF>(v);
+  v = dpp_min<0x142, 0xA>(v);
+  v = dpp_min<0x143, 0xC>(v);
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 // Sum over the block (every thread gets it); red holds a value a wave, of 16 at most.
 __device__ __forceinline__ u64 block_sum_u64(u64 v, u64* red) {
@@ -658,7 +678,8 @@ __device__ __forceinline__ void sr_store(const SampleRowsParams& p, int row, con
 }
 
 // 4. A block a row: the cut, and the draw where every token that stayed was gathered. Bound by the barriers and by
-// what every wave computes alike: 512 threads take 10.7 us for one row, 1024 12.7, 256 9.1; of 160 rows 20, 19, 26.
+// what every wave computes alike: 512 threads take 12.7 us for one row of 200 gathered tokens, 1024 15.6, 256 12.4; of
+// 160 rows 20, 19, 26. Up to 64 tokens one wave compares each with each: 4.2 us against 10.7.
 template <class T>
 __global__ __launch_bounds__(kSrRowThreads) void sample_cut_kernel(SampleRowsParams p) {
   __shared__ u64 key_s[kSrGather], mass_s[kSrGather];
@@ -704,6 +725,37 @@ __global__ __launch_bounds__(kSrRowThreads) void sample_cut_kernel(SampleRowsPar
     return;
   }
   const int n = min(st.gathered, kSrGather);
+  if (n <= 64) {
+    // A wave's worth: every token's place in the order by comparing it with each of the others, no barriers.
+    if (t >= 64) return;
+    const u64 key = t < n ? item[0] : 0;
+    u64 m = t < n ? sc.mass(sr_logit(key)) : 0, before = 0, total = st.total;
+    int rank = 0;
+    for (int i = 0; i < n; ++i) {
+      const u64 k = wave_lane_u64(key, i), w = wave_lane_u64(m, i);
+      rank += k > key && w;
+      before += k > key ? w : 0;
+    }
+    if (st.mode == SR_EDGE) {
+      const u64 want = (st.by_k ? (u64)s.top_k : sr_ceil(s.top_p, total)) - st.base;
+      if (m && (st.by_k ? (u64)rank + 1 == want : before < want && before + m >= want)) w.st->cut = key;
+      if (t == 0) w.st->mode = SR_DRAW;
+      return;
+    }
+    if (st.by_k) {
+      if (rank >= s.top_k) m = 0;
+      total = wave_sum_u64(m);
+    }
+    if (s.top_p < 1.f && before >= sr_ceil(s.top_p, total)) m = 0;
+    if (m < sc.floor_mass(s.min_p)) m = 0;
+    total = wave_sum_u64(m);
+    const u64 want = sr_target(st.u, total), place = key & (kSrMaxVocab - 1);
+    before = 0;
+    for (int i = 0; i < n; ++i) before += (wave_lane_u64(key, i) & (kSrMaxVocab - 1)) > place ? wave_lane_u64(m, i) : 0;
+    if (m && before <= want && want < before + m) sr_store(p, row, sc, s.temperature, sr_logit(key), sr_index(key), total);
+    if (t == 0) w.st->mode = SR_DONE;
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < OWN; ++i)
     if (t + i * kSrRowThreads < n) {
