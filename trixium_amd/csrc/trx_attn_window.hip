@@ -763,8 +763,8 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ * WK / 4) void attn_window_kernel(
 // keys at a time by itself, without barriers: its K rows come straight into the operand's registers, its V
 // rows through LDS of its own (to be read transposed), both one tile ahead; the queries, the same for
 // all four, lie in LDS to leave the registers to the rows. Bound by the rows' latency and
-// bytes, the joins and, for short windows, the two launches: one position over 32768 keys (134 MB) 32 us with
-// both launches, 4.2 TB/s; over 1024 keys (4.2 MB) 13.4, of which 10 and 3 are the two kernels.
+// bytes, the joins and, for short windows, the two launches: one position over 32768 keys (134 MB) 25 us, 5.4 TB/s,
+// and 6 in the second launch; over 1024 keys (4.2 MB) 9 and 3.
 template <int HD, bool HALF>
 __global__ __launch_bounds__(256, 1) void attn_window_few_kernel(AttnWindowParams p) {
   using Wave = AwWave<HD, HALF>;
@@ -1004,13 +1004,12 @@ struct AwPlan {
 // first rows' latency, the join of its waves, the outputs) and a step for each wk tiles of keys; a full chip
 // makes a step 1.4 times as long; splits write and read their sums once at 3 TB/s. Measured (us, by wq and
 // splits), the choice first:
-//   27 positions over 4061 keys, 32 heads of 128, 8 kv heads: (1, 8) 25.0; (2, 16) 24.9, (2, 4) 32, (4, 16) 28,
-//     (4, 1) 105, (1, 4) 33, (1, 16) 33
-//   1024 over windows of 2048: (4, 1) 91; (2, 1) 121, (1, 1) 200, (4, 2) 130
-//   509 over up to 1209 keys, 24 heads of 256, 4 kv heads: (4, 2) 79; (4, 1) 107, (2, 1) 86, (4, 3) 90, (1, 2) 120
-//   1 over 32768 keys, fp16 queries: (1, 32) 32; (1, 16) 46, (1, 24) 36, (1, 64) 45, (2, 32) 37
-//   200 over 4061 + 200 keys: (4, 4) 54; (2, 2) 57, (2, 4) 67, (4, 8) 70
-//   1 over 1024 keys, 16 heads: (1, 8) 14.8; (1, 4) 16.1, (1, 24) 15.2, (1, 64) 26
+//   27 positions over 4061 keys, 32 heads of 128, 8 kv heads: (1, 8) 20; (1, 6) 23, (2, 16) 23, (4, 32) 25, (1, 1) 68
+//   200 of them: (4, 4) 51; (2, 2) 53, (2, 4) 61, (1, 1) 71
+//   1024 over windows of 2048: (4, 1) 85; (4, 2) 105, (2, 1) 115, (1, 1) 155
+//   509 over up to 1209 keys, 24 heads of 256, 4 kv heads: (4, 2) 70; (4, 4) 78, (2, 1) 88, (1, 1) 93, (4, 1) 103
+//   1 over 32768 keys, fp16 queries: (1, 32) 32; (1, 24) 34, (2, 32) 36, (1, 1) 437
+//   1 over 1024 keys, 16 heads: (1, 8) 12; (1, 16) 13, (1, 4) 14, (1, 1) 24
 static AwPlan aw_plan(const AttnWindowParams& p, long long pos, int most) {
   const int rep = p.n_head / p.n_kv, cols = p.n * rep;
   AwPlan best = {1, 1};
@@ -1021,7 +1020,7 @@ static AwPlan aw_plan(const AttnWindowParams& p, long long pos, int most) {
     // A few-columns step waits for its own rows. Of the others' the matrix products are the larger part (two
     // planes of queries and probabilities with fp32); wq = 2 has one stage less on the way.
     const double unit = wq == 1 ? p.hd / 64.0 : 1.35 * (p.half_io ? 0.56 : 1.0) * (p.hd == 64 ? 0.6 : 1.0);
-    const double step = wq == 2 ? unit * (p.hd == 256 || p.half_io ? 1.7 : 1.3) : unit;
+    const double step = wq == 2 ? unit * (p.half_io ? 1.75 : p.hd == 256 ? 1.7 : 1.3) : unit;
     const long long span = std::min<long long>(p.n, (32 * wq + rep - 1) / rep + 1);
     const long long keys = std::min<long long>((long long)p.sinks + p.window + span - 1, pos + p.n);
     const int tiles = (int)((keys + kAwKeys - 1) / kAwKeys), blocks = cdiv(cols, 32 * wq) * p.n_kv;
