@@ -219,7 +219,7 @@ int trx_gemv_packed_parts_f32(const uint8_t* packed, int kind, int M, int K, con
  * r * kv_stride + g * head_dim. Strides are in elements: q_stride a multiple of 16 bytes, kv_stride of
  * 8 and at most 2^22, the others of 4; every pointer is 16-byte aligned.
  * head_dim 64, 128 or 256; 0 <= sinks <= pin < slots, 1 <= window <= slots - pin, scale > 0, n >= 0
- * (0: nothing is done).
+ * (0: nothing is done), n * n_head <= 2^25.
  * The ring holds the positions below pos that a query sees; slots that no visible position takes may
  * hold anything. Afterwards the new rows stand in their slots (of rows that share a slot, the last);
  * no other slot is written. An infinity or NaN in a key or value that a query does not see does not

@@ -156,6 +156,15 @@ def test_geometry_refuses(change, what):
     assert what in lib.trx_last_error()
 
 
+def test_geometry_refuses_more_positions_than_a_grid_holds():
+    shape = Case(32, 8, 128, slots=64, pin=4, window=60, sinks=4).c_shape()
+    size = ctypes.c_size_t()
+    geometry = _lib.lib().trx_attn_window_geometry
+    assert geometry(ctypes.byref(shape), 2**20, ctypes.byref(size)) == _lib.TRX_OK
+    assert geometry(ctypes.byref(shape), 2**20 + 1, ctypes.byref(size)) == _lib.TRX_E_INVALID
+    assert geometry(ctypes.byref(shape), -1, ctypes.byref(size)) == _lib.TRX_E_INVALID
+
+
 def test_call_refuses_bad_arguments():
     c = Case(4, 2, 64, 64, 4, 60, 4)
     lib, shape = _lib.lib(), c.c_shape()

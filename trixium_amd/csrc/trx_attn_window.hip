@@ -119,7 +119,7 @@ __device__ __forceinline__ uint32_t finite_h(uint32_t two) {
   return __builtin_bit_cast(uint32_t, x >> 15);
 }
 
-// The position's row of a column: column / rep by a product (columns below 2^28, rep_m = 2^rep_s / rep rounded up,
+// The position's row of a column: column / rep by a product (columns below 2^25, rep_m = 2^rep_s / rep rounded up,
 // 2^rep_s at least 2^32 rep: exact).
 __device__ __forceinline__ int aw_row(const AttnWindowParams& p, int column) {
   return (int)((unsigned long long)(unsigned)column * p.rep_m >> p.rep_s);
@@ -919,7 +919,7 @@ __global__ __launch_bounds__(256) void attn_window_finish(AttnWindowParams p, in
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   if ((int)blockIdx.x < join_blocks) {
     constexpr int E = HD / 64;                     // dims a lane: E lane .. + E - 1
-    const unsigned id = blockIdx.x * 4 + w;         // below 2^28 + 4
+    const unsigned id = blockIdx.x * 4 + w;         // below 2^25 + 4
     if (id >= (unsigned)(p.n * p.n_head)) return;
     const int row = (int)(id / (unsigned)p.n_head), head = (int)id - row * p.n_head, g = aw_row(p, head);
     const int col = row * p.rep + head - g * p.rep;
@@ -981,7 +981,7 @@ __global__ __launch_bounds__(256) void attn_window_finish(AttnWindowParams p, in
   const long long id = (long long)(blockIdx.x - join_blocks) * 256 + threadIdx.x;
   const long long pieces = (long long)p.n * p.n_kv * SEG;
   if (id >= pieces) return;
-  const unsigned at = (unsigned)(id / SEG);        // below 2^28
+  const unsigned at = (unsigned)(id / SEG);        // below 2^25
   const int sd = (int)(id % SEG) * 8, r = (int)(at / (unsigned)p.n_kv), g = (int)at - r * p.n_kv, u = pos + r;
   if (u >= p.pin && p.n - r > R) return;
   const int slot = u < p.pin ? u : p.pin + (int)((unsigned)(u - p.pin) % (unsigned)R);
@@ -1046,7 +1046,8 @@ const char* attn_window_refuses(const AttnWindowParams& p) {
   if (p.pin < 0 || p.slots <= p.pin) return "pin outside [0, slots)";
   if (p.sinks < 0 || p.sinks > p.pin) return "sinks outside [0, pin]";
   if (p.window < 1 || p.window > p.slots - p.pin) return "window outside [1, slots - pin]";
-  if (p.n < 0 || (long long)p.n * p.n_head > (1 << 28)) return "too many positions";
+  // (The second kernel's threads, up to 64 a position and head, stay below a grid's 2^32.)
+  if (p.n < 0 || (long long)p.n * p.n_head > (1 << 25)) return "too many positions";
   if (!(p.scale > 0.f && p.scale < INFINITY)) return "scale is not positive and finite";
   const int q4 = p.half_io ? 8 : 4, o4 = 4;
   if (p.q_stride < p.n_head * p.hd || p.q_stride % q4) return "q_stride";
