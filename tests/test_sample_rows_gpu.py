@@ -297,3 +297,22 @@ def test_rows_cut_into_long_chunks(vocab, n, dtype):
     assert np.array_equal(tok[some], again) and np.array_equal(lp[some], lp2)
     for r in some[:4]:
         assert oracle(lg[r], u[r], *(kw[k][r] for k in ROW.names))[0] == tok[r]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+def test_cuts_beside_tokens_without_mass(dtype):
+    """The cut lies in the histogram's last step, where the tokens too far below the largest stand as well."""
+    rng = np.random.default_rng(8)
+    vocab = 6000
+    lg = np.stack([rng.permutation(np.linspace(0, -60, vocab)) for _ in range(4)]).astype(dtype)
+    lg[3, 17] = lg[3, 4000] = np.inf
+    mass = [int(m) for m in np.rint(np.exp(lg[0].astype(np.float64)) * 2.0**_frac(vocab))]
+    live = sum(m > 0 for m in mass)
+    assert 1000 < live < vocab
+    us = np.array([0.2, 0.6, 1 - 2.0**-24, 0.7], np.float32)
+    for k in (live - 1, live, live + 1, live - 3):
+        check(lg, us, top_k=k)
+        check(lg, us, top_k=k, top_p=1 - 2.0**-24)
+    check(lg, us, top_p=1 - 2.0**-24)
+    check(lg, us, top_p=0.5, top_k=2)
