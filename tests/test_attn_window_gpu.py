@@ -487,3 +487,29 @@ def test_positions_up_to_the_largest(kind, heads, kv, hd, n):
         assert np.array_equal(x.view(np.uint8), y.view(np.uint8))
     with pytest.raises(_lib.TrxError):
         _call(c, q, k, v, kc, vc, pos=top + 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,hd,window,n", [(32, 8, 128, 60, 1), (6, 1, 256, 40, 5), (4, 2, 64, 50, 9),
+                                                  (8, 8, 128, 90, 31)])
+def test_few_columns_with_fp16_queries_round_once(heads, kv, hd, window, n):
+    """A token's or a short turn's fp16 outputs are the fp32 result rounded: x + d rounds to a value whose distance
+    from x is at most that of x rounded, plus 2 d. Queries with one element leave a score no sum over dims: d is
+    the fp32 tolerance without it."""
+    c = Case(heads, kv, hd, slots=window + 50, pin=4, window=window, sinks=4, kind=F16, seed=15, scale=1.0)
+    c.extend(window + 99)
+    pos = c.K.shape[0]
+    q, k, v = c.rows(n)
+    q[..., 1:] = 0
+    out, _, _ = _call(c, q, k, v, *c.ring())
+    out = out.reshape(n, heads, hd).astype(np.float64)
+    K, V = (np.concatenate(a).astype(np.float64) for a in ((c.K, k), (c.V, v)))
+    for r in range(n):
+        u = np.r_[:4, pos + r - window + 1:pos + r + 1]
+        for h in range(heads):
+            s = K[u, h * kv // heads, 0] * float(q[r, h, 0])
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            Vu = V[u, h * kv // heads]
+            x, d = p @ Vu, (p @ np.abs(Vu)) * (2 * (np.abs(s).max() + 1) * 2.0**-21 + u.size * 2.0**-24 + 2.0**-22)
+            assert (np.abs(out[r, h] - x) <= np.abs(x.astype(np.float16).astype(np.float64) - x) + 2 * d).all(), (r, h)

@@ -15,9 +15,11 @@
 //   S^T = K Q^T: fp32 queries enter as two fp16 planes of q * 2^e (e per query: the largest element
 //   below 2^14), so a score is the fp32 dot product to 2^-22; fp16 queries as they are.
 //   O^T += V^T P^T: P^T stands in the score registers in the operand's layout but for the order of
-//   the keys, which V^T, read transposed from LDS, follows. fp32 outputs: P in two fp16 planes
-//   (2^-22); fp16 outputs: one (2^-12 a probability at most, a quarter step of the output, and
-//   independent from key to key).
+//   the keys, which V^T, read transposed from LDS, follows. P in two fp16 planes (2^-22), but in one for
+//   fp16 outputs of many columns: 2^-11 a probability at most, as the output's own rounding, independent
+//   from key to key (against 64 bits 2.9e-4 of the result's norm, 2.1e-4 with two planes). The second plane
+//   is a third of the products: 1021 positions x 32 heads of 128 over 6000 keys 130 us with one, 164 with two;
+//   one position over 32768 keys 35.1 and 35.6.
 // Probabilities are 2^(s - r + 7) against a reference r that follows the running maximum only where
 // that exceeds it by 2^8: at most 2^15 (finite in fp16), and those that vanish in fp16 are below 2^-32
 // of the largest.
@@ -261,8 +263,8 @@ struct AwQuery {
   }
 };
 
-// A wave's running maximum, sums and outputs of its 32 columns.
-template <int HD, bool HALF>
+// A wave's running maximum, sums and outputs of its 32 columns. TWO: the probabilities' second plane.
+template <int HD, bool HALF, bool TWO>
 struct AwWave {
   static constexpr int NC = HD / 16, NDT = HD / 32;      // chunks of 16 dims; output tiles of 32
   f32x16_t o[NDT];
@@ -344,10 +346,10 @@ struct AwWave {
                             __builtin_amdgcn_exp2f(fmaf(s[8 * kh + 2 * i + 1], cs, ref))};
         l += pe.x + pe.y;
         hi[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(pe, half2v_t));
-        if constexpr (!HALF) lw[i] = rest_h(hi[i], pe.x, pe.y);
+        if constexpr (TWO) lw[i] = rest_h(hi[i], pe.x, pe.y);
       }
       ph[kh] = __builtin_bit_cast(half8_t, u32x4_t{hi[0], hi[1], hi[2], hi[3]});
-      if constexpr (!HALF) pl[kh] = __builtin_bit_cast(half8_t, u32x4_t{lw[0], lw[1], lw[2], lw[3]});
+      if constexpr (TWO) pl[kh] = __builtin_bit_cast(half8_t, u32x4_t{lw[0], lw[1], lw[2], lw[3]});
     }
   }
 
@@ -366,7 +368,7 @@ struct AwWave {
       for (int kh = 0; kh < 2; ++kh) {
         const half8_t a = values(tr, dt, kh);
         o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[kh], o[dt], 0, 0, 0);
-        if constexpr (!HALF) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[kh], o[dt], 0, 0, 0);
+        if constexpr (TWO) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[kh], o[dt], 0, 0, 0);
       }
   }
 
@@ -386,7 +388,7 @@ struct AwWave {
         }
         const half8_t a = __builtin_bit_cast(half8_t, raw);
         o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[kh], o[dt], 0, 0, 0);
-        if constexpr (!HALF) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[kh], o[dt], 0, 0, 0);
+        if constexpr (TWO) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[kh], o[dt], 0, 0, 0);
       }
   }
 
@@ -569,7 +571,7 @@ __device__ __forceinline__ uint32_t aw_tr(uint32_t tile, int lane) {
 // 95 against 88 us, and 15 us of 115 with 256 dims, where it had cost spilled registers.
 template <int HD, bool HALF, int WQ, int WK, int D>
 __global__ __launch_bounds__(64 * WQ * WK, WQ * WK / 4) void attn_window_kernel(AttnWindowParams p) {
-  using Wave = AwWave<HD, HALF>;
+  using Wave = AwWave<HD, HALF, !HALF>;
   using Lds = AwLds<HD>;
   constexpr int NW = WQ * WK;
   constexpr int SR = WK * kAwKeys;                // keys a stage
@@ -767,7 +769,7 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ * WK / 4) void attn_window_kernel(
 // and 6 in the second launch; over 1024 keys (4.2 MB) 9 and 3.
 template <int HD, bool HALF>
 __global__ __launch_bounds__(256, 1) void attn_window_few_kernel(AttnWindowParams p) {
-  using Wave = AwWave<HD, HALF>;
+  using Wave = AwWave<HD, HALF, true>;
   using Lds = AwLds<HD>;
   constexpr int WK = 4, SEG = HD / 8;
   constexpr int PP = kAwKeys * SEG / 64, RPP = 64 / SEG;  // a lane's 16-byte pieces of V; rows between them
