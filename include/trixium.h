@@ -228,8 +228,8 @@ int trx_gemv_packed_parts_f32(const uint8_t* packed, int kind, int M, int K, con
  * pos_dev != NULL: the first position is read from the device when the work runs (for captured
  * graphs) and `pos` is ignored; a position there that is negative or leaves int32 within n leaves out
  * and the ring as they are.
- * workspace: trx_attn_window_geometry's bytes (may be 0: NULL then), no zeroing needed; calls that
- * share it must not overlap. */
+ * workspace: trx_attn_window_geometry's bytes for n, which hold any call of the shape of up to n
+ * positions (may be 0: NULL then), no zeroing needed; calls that share it must not overlap. */
 typedef struct trx_attn_window_shape {
   int kind;
   int n_head, n_kv_head, head_dim;

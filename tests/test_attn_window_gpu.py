@@ -513,3 +513,60 @@ def test_few_columns_with_fp16_queries_round_once(heads, kv, hd, window, n):
             Vu = V[u, h * kv // heads]
             x, d = p @ Vu, (p @ np.abs(Vu)) * (2 * (np.abs(s).max() + 1) * 2.0**-21 + u.size * 2.0**-24 + 2.0**-22)
             assert (np.abs(out[r, h] - x) <= np.abs(x.astype(np.float16).astype(np.float64) - x) + 2 * d).all(), (r, h)
+
+
+# The workspace of a length holds every shorter one's --------------------------------------------------
+
+
+@pytest.mark.parametrize("kind", [F32, F16])
+@pytest.mark.parametrize("heads,kv,hd,window", [(32, 8, 128, 2048), (32, 8, 128, 4092), (24, 4, 256, 2044), (16, 8, 128, 1020),
+                                                (4, 2, 64, 124), (64, 4, 64, 30000), (1, 1, 256, 1 << 20)])
+def test_the_workspace_does_not_shrink_with_the_length(heads, kv, hd, window, kind):
+    """geometry(n) is a bound for every call of up to n positions: it never falls as n grows, and below 64
+    positions (each length's own figure) it is the largest so far."""
+    shape = Case(heads, kv, hd, slots=window + 4, pin=4, window=window, sinks=4, kind=kind).c_shape()
+    lengths = list(range(1, 700)) + [2**k + d for k in range(10, 15) for d in (-1, 0, 1, 17)]
+    sizes = [_geometry(shape, n) for n in lengths]
+    assert sizes == sorted(sizes)
+    assert _geometry(shape, 0) == 0
+    assert all(s % (heads * (hd + 2) * 4) == 0 for s in sizes)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F32, F16])
+@pytest.mark.parametrize("heads,kv,hd,window,longest", [(32, 8, 128, 2048, 700), (24, 4, 256, 2044, 700), (4, 2, 64, 900, 300)])
+def test_one_workspace_for_a_prompt_and_its_rest(heads, kv, hd, window, longest, kind):
+    """Sized for the longest call, used by shorter ones, whose keys may be split further: nothing is written behind
+    it, and the results are those of a workspace of their own."""
+    c = Case(heads, kv, hd, slots=window + 4, pin=4, window=window, sinks=4, kind=kind, seed=16)
+    _, kc, vc = c.rows(c.slots)
+    kc, vc = (np.ascontiguousarray(a.transpose(1, 0, 2)) for a in (kc, vc))
+    B, shape, guard = _lib.DeviceBuffer, c.c_shape(), 1 << 20
+    size = _geometry(shape, longest)
+    work = B.from_array(np.full(size + guard, 0xA5, np.uint8))
+    for n in (longest, 400, 300, 256, 200, 129, 64, 27, 3, 1):
+        if n > longest:
+            continue
+        q, k, v = c.rows(n)
+        want = _call(c, q, k, v, kc, vc, pos=3 * window)
+        qb, kn, vn, kb, vb = (B.from_array(a) for a in (q, k, v, kc, vc))
+        out = B(q.nbytes)
+        _lib.call("trx_attn_window", ctypes.byref(shape), n, 3 * window, None, qb.ptr, kn.ptr, vn.ptr, kb.ptr, vb.ptr, None,
+                  out.ptr, work.ptr, None)
+        _lib.synchronize()
+        assert np.array_equal(out.download(np.uint8, q.nbytes), want[0].view(np.uint8).ravel()), n
+        assert (work.download(np.uint8, guard, offset=size) == 0xA5).all(), n
+
+
+@pytest.mark.gpu
+def test_kv_ring_object_keeps_its_workspace():
+    """A long chunk, then shorter ones and single tokens over the same object."""
+    from trixium_amd.attention import KVRing
+    c = Case(4, 2, 64, 1004, 4, 1000, 4, seed=17)
+    ring = KVRing(4, 2, 64, 1004)
+    for n in (1, 900, 300, 27, 1):
+        q, k, v = c.rows(n)
+        want, tol = c.expect(q, k, v)
+        assert (np.abs(ring.attend(q, k, v) - want) <= tol).all()
+        c.K, c.V = np.concatenate([c.K, k]), np.concatenate([c.V, v])
+    assert ring.work_n == 900 and ring.work.nbytes == _geometry(ring.shape, 900) >= _geometry(ring.shape, 300)

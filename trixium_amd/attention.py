@@ -34,7 +34,7 @@ class KVRing:
             window=int(self.slots - pin if window is None else window), sinks=int(pin if sinks is None else sinks),
             q_stride=q, kv_stride=kv, out_stride=q, gate_stride=q, gate_head_stride=self.hd,
             scale=1.0 / math.sqrt(self.hd) if scale is None else scale)
-        self.work = None
+        self.work, self.work_n = None, 0           # the workspace, of calls of up to work_n positions
         self._workspace(1)                         # refuses an unsupported shape before any allocation
         self.position = 0                          # of the next row
         self.kcache = _lib.DeviceBuffer(2 * kv * self.slots)
@@ -44,11 +44,13 @@ class KVRing:
         _lib.synchronize()
 
     def _workspace(self, n):
-        size = ctypes.c_size_t()
-        _lib.call("trx_attn_window_geometry", ctypes.byref(self.shape), n, ctypes.byref(size))
-        if size.value and (self.work is None or self.work.nbytes < size.value):
-            self.work = _lib.DeviceBuffer(size.value)
-        return self.work.ptr if size.value else None
+        if n > self.work_n:
+            size = ctypes.c_size_t()
+            _lib.call("trx_attn_window_geometry", ctypes.byref(self.shape), n, ctypes.byref(size))
+            if size.value and (self.work is None or self.work.nbytes < size.value):
+                self.work = _lib.DeviceBuffer(size.value)
+            self.work_n = n
+        return self.work.ptr if self.work else None
 
     def attend(self, q, k, v, gate=None):
         """Outputs [n, n_head, head_dim] of the next n positions: q (and gate) [n, n_head, head_dim], k

@@ -25,7 +25,7 @@ struct AttnWindowParams {
   int n_head, n_kv, hd, slots, pin, window, sinks;
   int q_stride, kv_stride, out_stride, gate_stride, gate_head_stride;
   float scale;
-  void* work;                  // attn_window_work_bytes
+  void* work;                  // attn_window_work_bytes (null where the call splits no keys)
   // Set by the launcher.
   int rep, nsplit, cols;       // heads a kv head; splits of the keys; n * rep
   unsigned long long rep_m;    // for the division by rep: a product with rep_m, shifted by rep_s
@@ -34,7 +34,9 @@ struct AttnWindowParams {
 
 // Why a geometry is not taken (null: it is).
 const char* attn_window_refuses(const AttnWindowParams& p);
+// Bytes that any call of up to p.n positions needs; and whether the one of p.n needs any.
 size_t attn_window_work_bytes(const AttnWindowParams& p);
+bool attn_window_splits(const AttnWindowParams& p);
 int launch_attn_window(const AttnWindowParams& p, hipStream_t s);
 
 }  // namespace trx

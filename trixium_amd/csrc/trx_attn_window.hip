@@ -1061,11 +1061,40 @@ const char* attn_window_refuses(const AttnWindowParams& p) {
   return nullptr;
 }
 
-size_t attn_window_work_bytes(const AttnWindowParams& p) {
-  if (p.n == 0) return 0;
-  const int s = aw_plan(p, LLONG_MAX / 2, kAwMaxSplits).nsplit;
-  return s > 1 ? (size_t)s * p.n * p.n_head * (p.hd + 2) * 4 : 0;
+// Lengths in steps of 1/64 to 1/32 of them (of one below 64). A call takes at most as many split positions, n times
+// the splits, as the calls at both ends of its step would at the step's last length: so the workspace of a length
+// holds that of every shorter one (the splits fall as n grows, and with them, here and there, the bytes). Of 1.3
+// million calls (1 to 9000 positions, windows of 30 to 131068, 1 to 128 heads) that takes splits from 424, by the
+// estimate at most 1% slower for it.
+static int aw_step(int n) {
+  int step = 1;
+  while (64ll * step <= n) step *= 2;
+  return step;
 }
+static long long aw_split_positions(AttnWindowParams p, int first, int step) {
+  int s = 1;
+  for (int n : {first, first + step - 1}) {
+    p.n = n;
+    s = std::max(s, aw_plan(p, LLONG_MAX / 2, kAwMaxSplits).nsplit);
+  }
+  return s > 1 ? (long long)s * (first + step - 1) : 0;
+}
+// The cut of a call whose windows are full.
+static AwPlan aw_full_plan(const AttnWindowParams& p) {
+  const AwPlan plan = aw_plan(p, LLONG_MAX / 2, kAwMaxSplits);
+  const int step = aw_step(p.n);
+  if (step == 1 || plan.nsplit == 1) return plan;
+  const long long most = aw_split_positions(p, p.n / step * step, step) / p.n;
+  return plan.nsplit <= most ? plan : aw_plan(p, LLONG_MAX / 2, (int)std::max(most, 1ll));
+}
+
+// Of any call of up to n positions.
+size_t attn_window_work_bytes(const AttnWindowParams& p) {
+  long long most = 0;
+  for (int n = 1; n <= p.n; n += aw_step(n)) most = std::max(most, aw_split_positions(p, n, aw_step(n)));
+  return (size_t)most * p.n_head * (p.hd + 2) * 4;
+}
+bool attn_window_splits(const AttnWindowParams& p) { return p.n > 0 && aw_full_plan(p).nsplit > 1; }
 
 template <int HD, bool HALF>
 static int aw_launch(const AttnWindowParams& p, int wq, hipStream_t s) {
@@ -1093,7 +1122,7 @@ int launch_attn_window(const AttnWindowParams& params, hipStream_t s) {
   while (1 << (p.rep_s - 32) < p.rep) ++p.rep_s;
   p.rep_m = ((1ull << p.rep_s) + p.rep - 1) / p.rep;
   // The workspace holds the splits of a full window; a ring that is still filling takes no more.
-  AwPlan plan = aw_plan(p, LLONG_MAX / 2, kAwMaxSplits);
+  AwPlan plan = aw_full_plan(p);
   if (!p.pos_dev && p.pos < (long long)p.sinks + p.window) plan = aw_plan(p, p.pos, plan.nsplit);
   p.nsplit = plan.nsplit;
   if (p.half_io) {
@@ -1160,7 +1189,7 @@ TRX_API int trx_attn_window(const trx_attn_window_shape* shape, int n, int pos, 
   TRX_CHECK(q && k && v && kcache && vcache && out, TRX_E_INVALID, "trx_attn_window: null argument");
   TRX_CHECK(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(kcache) && aligned16(vcache) && aligned16(gate) &&
             aligned16(out) && aligned16(workspace), TRX_E_INVALID, "trx_attn_window: a pointer is not 16-byte aligned");
-  TRX_CHECK(workspace || attn_window_work_bytes(p) == 0, TRX_E_INVALID, "trx_attn_window: null workspace");
+  TRX_CHECK(workspace || !attn_window_splits(p), TRX_E_INVALID, "trx_attn_window: null workspace");
   p.q = q;
   p.out = out;
   p.k = (const __half*)k;

@@ -1692,8 +1692,6 @@ TRX_API int trx_model_prefill(trx_model* h, int n, int chunk) {
   const int part = std::min(chunk, n - n_in);
   if (part >= kRowsMin && rows_take(m, part, 0)) {
     if ((rc = pf_alloc(m, part)) == TRX_OK) rc = ring_alloc(m, part);
-    const int tail = (n - n_in) % part;              // the last chunk may split its keys further
-    if (rc == TRX_OK && tail) rc = ring_alloc(m, tail);
     if (rc != TRX_OK && rc != TRX_E_NOMEM) return rc;
     for (; rc == TRX_OK && done < n; done += std::min(part, n - done)) {
       const int R = std::min(part, n - done);
