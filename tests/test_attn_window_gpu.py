@@ -570,3 +570,55 @@ def test_kv_ring_object_keeps_its_workspace():
         assert (np.abs(ring.attend(q, k, v) - want) <= tol).all()
         c.K, c.V = np.concatenate([c.K, k]), np.concatenate([c.V, v])
     assert ring.work_n == 900 and ring.work.nbytes == _geometry(ring.shape, 900) >= _geometry(ring.shape, 300)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F32, F16])
+@pytest.mark.parametrize("heads,kv,hd,window,n", [(4, 2, 64, 2300, 1), (4, 2, 128, 200, 1), (6, 1, 256, 200, 9),
+                                                  (64, 4, 128, 600, 140), (64, 4, 64, 1000, 140), (64, 8, 256, 333, 140),
+                                                  (16, 4, 128, 2300, 180)])
+def test_a_seen_infinity_far_below_the_largest_score(kind, heads, kv, hd, window, n):
+    """One key's score is 860 powers of two above the others', whose probabilities vanish: the outputs are that
+    key's values, and an infinity among the others' is an infinity, wherever the keys are cut into waves and
+    splits. With fp16 queries some scores are -inf, a whole tile of them beside the infinity."""
+    c = Case(heads, kv, hd, slots=window + 200, pin=4, window=window, sinks=4, kind=kind, seed=13, scale=1.0)
+    c.extend(window + 250)
+    c.K[:] = 0
+    q, k, v = c.rows(n)
+    q[:], k[:] = 0, 0
+    q[..., 0] = 10
+    pos, seen = c.K.shape[0], 250 + n - 1 + 4              # the first position that every query sees, and some
+    top = pos - 40
+    c.K[top, :, 0] = 60
+    at = [2] + list(range(seen, top - 1, max(1, (top - seen) // 24)))
+    for i, u in enumerate(at):
+        c.V[u, :, 3 + i], c.V[u, :, hd - 1 - i] = np.inf, -np.inf
+    if kind == F16:
+        c.K[at[5] - 40:at[5] + 41, :, 0] = -np.inf
+    kc, vc = c.ring()
+    out, _, _ = _call(c, q, k, v, kc, vc)
+    out = out.reshape(n, heads, hd).astype(np.float64)
+    want = np.repeat(np.broadcast_to(c.V[top].astype(np.float64), (n, kv, hd)), heads // kv, axis=1).copy()
+    for i in range(len(at)):
+        want[..., 3 + i], want[..., hd - 1 - i] = np.inf, -np.inf
+    bad = np.isinf(want)
+    assert np.array_equal(out[bad], want[bad]), np.argwhere(bad & (out != want))[:6].tolist()
+    # Sums of one term: its probability's planes (2^-22, or 2^-11), 1 / l and the product (2^-24 each), the result.
+    eps = 2.0**-21 + (2.0**-10 if kind == F16 else 0)
+    assert (np.abs(out[~bad] - want[~bad]) <= eps * np.abs(want[~bad])).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F32, F16])
+@pytest.mark.parametrize("heads,kv,hd,window,n", [(32, 8, 128, 4000, 1), (32, 8, 128, 4000, 27), (24, 4, 256, 1500, 301),
+                                                  (64, 4, 64, 1000, 140)])
+def test_repeated_calls_give_the_same_bits(kind, heads, kv, hd, window, n):
+    """Over a ring whose replaced rows no query sees, the same call again gives the same outputs and ring."""
+    c = Case(heads, kv, hd, slots=window + n + 4, pin=4, window=window, sinks=4, kind=kind, seed=14)
+    q, k, v = c.rows(n)
+    _, kc, vc = c.rows(c.slots)
+    kc, vc = (np.ascontiguousarray(a.transpose(1, 0, 2)) for a in (kc, vc))
+    first = _call(c, q, k, v, kc, vc, pos=2 * window)
+    for _ in range(4):
+        for a, b in zip(first, _call(c, q, k, v, first[1], first[2], pos=2 * window)):
+            assert np.array_equal(a.view(np.uint8), b.view(np.uint8))

@@ -263,6 +263,10 @@ struct AwQuery {
   }
 };
 
+// A part's sum to the reference that the parts are joined at. An infinity (add_seen's) or NaN stays where the
+// factor has vanished: their product is NaN, whatever the parts that the keys were cut into.
+__device__ __forceinline__ float aw_rescaled(float x, float f) { return fabsf(x) < INFINITY ? x * f : x; }
+
 // A wave's running maximum, sums and outputs of its 32 columns. TWO: the probabilities' second plane.
 template <int HD, bool HALF, bool TWO>
 struct AwWave {
@@ -469,7 +473,7 @@ struct AwWave {
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) o[dt][e] *= f0;
+      for (int e = 0; e < 16; ++e) o[dt][e] = aw_rescaled(o[dt][e], f0);
 #pragma unroll 1
     for (int i = 0; i < WK - 1; ++i) {
       const float* b = jb + (size_t)(i * WQ + wq) * W * 64 + lane;
@@ -479,7 +483,7 @@ struct AwWave {
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[dt][e] += b[(dt * 16 + e) * 64] * fi;
+        for (int e = 0; e < 16; ++e) o[dt][e] += aw_rescaled(b[(dt * 16 + e) * 64], fi);
     }
     mref = M;
     return true;
@@ -904,7 +908,7 @@ __global__ __launch_bounds__(256, 1) void attn_window_few_kernel(AttnWindowParam
 #pragma unroll
     for (int i = 0; i < WK; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] += jb[((size_t)i * Wave::W + dt * 16 + e) * 64] * f[i];
+      for (int e = 0; e < 16; ++e) x[e] += aw_rescaled(jb[((size_t)i * Wave::W + dt * 16 + e) * 64], f[i]);
 #pragma unroll
     for (int a4 = 0; a4 < 4; ++a4)
       Wave::put(p, b, b.c0 + j, c.row, c.head, dt * 32 + 8 * a4 + 4 * h,
@@ -958,13 +962,13 @@ __global__ __launch_bounds__(256) void attn_window_finish(AttnWindowParams p, in
       M = top;
       l *= keep;
 #pragma unroll
-      for (int i = 0; i < E; ++i) o[i] *= keep;
+      for (int i = 0; i < E; ++i) o[i] = aw_rescaled(o[i], keep);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const float f = a[k].x == -INFINITY ? 0.f : a[k].x == M ? 1.f : __builtin_amdgcn_exp2f(a[k].x - M);
         l += a[k].y * f;
 #pragma unroll
-        for (int i = 0; i < E; ++i) o[i] += x[k][i] * f;
+        for (int i = 0; i < E; ++i) o[i] += aw_rescaled(x[k][i], f);
       }
     }
     const float inv = 1.0f / l;
