@@ -404,7 +404,8 @@ int trx_model_reset(trx_model* m);
  * work enqueued so far (position, fed and generated tokens, argmax slot, sampler stream, every
  * DeltaNet layer's conv window and recurrent matrix) into a buffer of the model (allocated on the
  * first save: the DeltaNet state's size, 151 MB at the 27B hybrid's shape); TRX_CKPT_RESTORE
- * enqueues the copy back, and the next forwards give the results they gave after the save. The KV
+ * enqueues the copy back, and the next forwards give the results they gave after the save, under
+ * the sampler set last (its settings are not state: a sampler set since the save stays set). The KV
  * rows are not copied: a forward writes its own position's row, so rows past the restored
  * position are rewritten before they are read. Outputs of the last forward (logits, taps) are not
  * state and are not restored. Asynchronous on the model's stream; TRX_E_STATE restores with no

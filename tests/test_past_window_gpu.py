@@ -209,3 +209,35 @@ def test_chat_goes_on_past_the_window(tiny_images):
     assert dec.position() > CAP
     with pytest.raises(ValueError):
         chat.reply("w " * (CAP + 1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("before,after", [
+    (dict(temperature=0.0), dict(temperature=1.5)),
+    (dict(temperature=0.9, top_k=1), dict(temperature=1.5)),
+    (dict(temperature=0.0), dict(temperature=0.0, repetition=1e30)),
+    (dict(temperature=1.5), "firmware"),
+    ("firmware", dict(temperature=1.5, repetition=1.2))], ids=str)
+def test_a_checkpoint_leaves_the_sampler_as_it_was_set_since(tiny_images, golden, before, after):
+    """The random stream is part of the state, the settings are not: after a restore the sampler set since the
+    checkpoint draws, and draws what it drew after the checkpoint."""
+    name = "tiny-qwen3"
+    dec = _decoder(tiny_images[(name, True)], max_new=32)
+
+    def choose(s):
+        if s == "firmware":
+            dec.set_sampling(1.4, 1.0, 1.3)
+        else:
+            dec.set_vocab_sampling(**s)
+
+    dec.set_vocab_sampling(temperature=1.0, seed=31)      # the stream
+    choose(before)
+    dec.reset()
+    dec.generate(golden[f"prompt/{name}"], 3)
+    dec.checkpoint()
+    choose(after)
+    a = dec.generate([1], 12)
+    dec.restore()
+    assert dec.generate([1], 12) == a
+    assert len(set(a)) > 4                                # drawn, or penalised: not the greedy repeats
+    dec.close()

@@ -1511,8 +1511,9 @@ TRX_API int trx_model_reset(trx_model* h) {
 }
 
 // The device regions a forward reads and rewrites from one position to the next: the control words
-// with the fed and generated tokens, the argmax slot, the sampler's settings, stream and candidates,
-// and every DeltaNet layer's conv window and recurrent matrix. The KV rows are not among them: a
+// with the fed and generated tokens, the argmax slot, the sampler's stream and candidates (not its settings:
+// the host's record of the sampler, which the launches follow, is of the last call that set it), and every
+// DeltaNet layer's conv window and recurrent matrix. The KV rows are not among them: a
 // forward appends the row of its own position, so rows past a restored position are written again
 // before any forward reads them.
 struct StateRegion {
@@ -1523,7 +1524,7 @@ static std::vector<StateRegion> state_regions(Model& m) {
   const trx_model_config& c = m.cfg;
   std::vector<StateRegion> r = {{m.ctl, (size_t)(8 + m.prompt_ring + c.max_new) * 4},
                                 {m.slot, 8},
-                                {m.smp, kSmpBytes},
+                                {m.smp + 3, 4},
                                 {m.smp_cand, 33 * 8}};
   if (m.n_dn) {
     const int nq = c.dn_num_k_heads * c.dn_k_head_dim, nvh = c.dn_num_v_heads * c.dn_v_head_dim;

@@ -315,7 +315,8 @@ class Decoder:
 
     def restore(self):
         """Put the last checkpoint's state back: the next forwards give the results they gave
-        after checkpoint() (KV rows past the position are rewritten before they are read)."""
+        after checkpoint(), under the sampler set last (KV rows past the position are rewritten
+        before they are read)."""
         _lib.call("trx_model_checkpoint", self._h, CKPT_RESTORE)
 
     def feed(self, tokens, head_from=-1):
