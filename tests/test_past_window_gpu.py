@@ -241,3 +241,20 @@ def test_a_checkpoint_leaves_the_sampler_as_it_was_set_since(tiny_images, golden
     assert dec.generate([1], 12) == a
     assert len(set(a)) > 4                                # drawn, or penalised: not the greedy repeats
     dec.close()
+
+
+@pytest.mark.gpu
+def test_more_heads_than_the_window_attention_takes():
+    """A model past the window attention's 1024 heads is stepped there, as one position a forward."""
+    from trixium_amd.model import Decoder
+    mc = C.TINY.replace(name="tiny-wide", n_head=1040, n_kv_head=130, n_layer=2, max_ctx=40)
+    rng = np.random.default_rng(2)
+    feeds = [rng.integers(0, mc.vocab, n).tolist() for n in (30, 25)]
+    out = []
+    for chunk in (0, 16):
+        dec = Decoder.synthetic(mc, seed=3, prefill_chunk=chunk)
+        dec.set_kv_ring(1, 4)
+        dec.reset()
+        out.append([dec.forward(f) for f in feeds])
+        dec.close()
+    assert max(_rel_err(b, a) for a, b in zip(*out)) <= 2e-3

@@ -1691,7 +1691,7 @@ TRX_API int trx_model_prefill(trx_model* h, int n, int chunk) {
   }
   int done = n_in;
   const int part = std::min(chunk, n - n_in);
-  if (part >= kRowsMin && rows_take(m, part, 0)) {
+  if (part >= kRowsMin && rows_take(m, part, 0) && (!m.n_attn || !attn_window_refuses(ring_attention(m, 0, part)))) {
     if ((rc = pf_alloc(m, part)) == TRX_OK) rc = ring_alloc(m, part);
     if (rc != TRX_OK && rc != TRX_E_NOMEM) return rc;
     for (; rc == TRX_OK && done < n; done += std::min(part, n - done)) {
