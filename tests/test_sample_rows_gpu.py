@@ -316,3 +316,20 @@ def test_cuts_beside_tokens_without_mass(dtype):
         check(lg, us, top_k=k, top_p=1 - 2.0**-24)
     check(lg, us, top_p=1 - 2.0**-24)
     check(lg, us, top_p=0.5, top_k=2)
+
+
+@pytest.mark.gpu
+def test_many_tokens_at_the_last_mass_of_none():
+    """The smallest logits stand exactly where a mass is half a unit, which rounds to none, and share the
+    histogram's last step with the cut: more of them than a gather holds must not push the others out. (The row's
+    largest logit comes last, and is drawn: everything else is below 2^-46 of the mass.)"""
+    vocab, T = 9000, np.float32(float.fromhex("0x1.00000ep-1"))
+    top, low = (float.fromhex(v) for v in ("0x1.0fb6c4p+4", "0x1.c22362p-22"))
+    c2 = 1.44269504088896340736 / np.float64(T)
+    assert np.float32(low) == low and (_frac(vocab) + 1) / c2 == top - low and (low - top) * c2 == -(_frac(vocab) + 1)
+    lg = np.full((8, vocab), low, np.float32)
+    lg[:, -1] = top
+    lg[:, 100:104] = low + np.array([1e-3, 2e-3, 3e-3, 4e-3])
+    us = np.linspace(0, 1 - 2.0**-24, 8).astype(np.float32)
+    for kw in (dict(top_k=2), dict(top_k=3), dict(top_k=3, min_p=0.1), dict(top_k=2, top_p=0.999)):
+        assert (check(lg, us, temperature=T, **kw) == vocab - 1).all()

@@ -122,8 +122,10 @@ struct SrScale {
     top = M;
     inf = M == INFINITY;
     c2 = 1.44269504088896340736 / (double)T;
-    const double reach = fmin((frac + 1) / c2, top - (double)low);   // below it a mass is 0
-    dead = inf || reach < top - (double)low;
+    const double end = (frac + 1) / c2;         // a mass of half a unit: below it, and rounded there, 0
+    const double reach = fmin(end, top - (double)low);
+    // (A mass above half a unit by 2^-36 of itself is one in spite of the roundings of y and of the series.)
+    dead = inf || !(top - (double)low < end * (1.0 - 0x1p-40));
     per = !inf && reach > 0.0 ? kSrBuckets / reach : 0.0;
   }
   __device__ __forceinline__ u64 mass(float l) const {
