@@ -148,6 +148,20 @@ def test_refusals():
     assert sample(np.zeros((0, 4), np.float32), [])[0].size == 0
 
 
+def test_a_top_k_past_int32_is_off(monkeypatch):
+    """2^32 + 5 is past every vocabulary, not 5."""
+    assert settings(top_k=[2**32 + 5, -2**33 + 7, 7, 0])["top_k"].tolist() == [2**31 - 1, -1, 7, 0]
+    assert settings(top_k=2**40 + 1)["top_k"].tolist() == [2**31 - 1]
+    from trixium_amd.model import Decoder
+    seen = []
+    monkeypatch.setattr(_lib, "call", lambda name, *a: seen.append(a[2]))
+    dec = Decoder.__new__(Decoder)
+    dec._h = None
+    for k in (2**32 + 5, -2**33 + 7, 40, 0):
+        dec.set_vocab_sampling(top_k=k)
+    assert seen[:4] == [2**31 - 1, -1, 40, 0]
+
+
 # Results (GPU) ---------------------------------------------------------------------------------------
 
 

@@ -287,7 +287,8 @@ class Decoder:
         the largest probability (0, 1 and 0 are off), one number of the firmware's xorshift32 stream a token
         (seed 0 keeps it). set_sampling's firmware sampler draws among 32 candidates; the last of the two
         calls counts, and set_sampling() is the greedy argmax again."""
-        _lib.call("trx_model_set_vocab_sampling", self._h, float(temperature), int(top_k), float(top_p), float(min_p),
+        top_k = min(max(int(top_k), -1), 2**31 - 1)
+        _lib.call("trx_model_set_vocab_sampling", self._h, float(temperature), top_k, float(top_p), float(min_p),
                   float(repetition), int(seed) & 0xFFFFFFFF)
 
     # State and decoding ------------------------------------------------------------------------
