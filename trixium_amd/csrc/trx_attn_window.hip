@@ -263,9 +263,12 @@ struct AwQuery {
   }
 };
 
-// A part's sum to the reference that the parts are joined at. An infinity (add_seen's) or NaN stays where the
-// factor has vanished: their product is NaN, whatever the parts that the keys were cut into.
-__device__ __forceinline__ float aw_rescaled(float x, float f) { return fabsf(x) < INFINITY ? x * f : x; }
+// What takes a part's sums from its reference to the larger one that the parts are joined at. Never 0, so that
+// an infinity (add_seen's) stays one where the part's largest score lies far below, or is -inf: a finite sum is
+// below 2^57, and what 2^-126 leaves of it far below the other parts' rounding. A part without a key: its sums are 0.
+__device__ __forceinline__ float aw_rescale(float from, float to) {
+  return from == to ? 1.f : fmaxf(__builtin_amdgcn_exp2f(from - to), 0x1p-126f);
+}
 
 // A wave's running maximum, sums and outputs of its 32 columns. TWO: the probabilities' second plane.
 template <int HD, bool HALF, bool TWO>
@@ -467,23 +470,21 @@ struct AwWave {
     float M = mref;
 #pragma unroll
     for (int i = 0; i < WK - 1; ++i) M = fmaxf(M, jb[((size_t)(i * WQ + wq) * W + W - 2) * 64 + lane]);
-    // A wave that saw no key leaves nothing (its sums are zero).
-    const float f0 = mref == M ? 1.f : mref == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mref - M);
+    const float f0 = aw_rescale(mref, M);
     l *= f0;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) o[dt][e] = aw_rescaled(o[dt][e], f0);
+      for (int e = 0; e < 16; ++e) o[dt][e] *= f0;
 #pragma unroll 1
     for (int i = 0; i < WK - 1; ++i) {
       const float* b = jb + (size_t)(i * WQ + wq) * W * 64 + lane;
-      const float mi = b[(W - 2) * 64];
-      const float fi = mi == -INFINITY ? 0.f : mi == M ? 1.f : __builtin_amdgcn_exp2f(mi - M);
+      const float fi = aw_rescale(b[(W - 2) * 64], M);
       l += b[(W - 1) * 64] * fi;
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[dt][e] += aw_rescaled(b[(dt * 16 + e) * 64], fi);
+        for (int e = 0; e < 16; ++e) o[dt][e] += b[(dt * 16 + e) * 64] * fi;
     }
     mref = M;
     return true;
@@ -893,8 +894,7 @@ __global__ __launch_bounds__(256, 1) void attn_window_few_kernel(AttnWindowParam
   for (int i = 0; i < WK; ++i) M = fmaxf(M, f[i] = jb[((size_t)i * Wave::W + Wave::W - 2) * 64]);
 #pragma unroll
   for (int i = 0; i < WK; ++i) {
-    // A wave that saw no key leaves nothing (its sums are zero).
-    f[i] = f[i] == -INFINITY ? 0.f : f[i] == M ? 1.f : __builtin_amdgcn_exp2f(f[i] - M);
+    f[i] = aw_rescale(f[i], M);
     l += jb[((size_t)i * Wave::W + Wave::W - 1) * 64] * f[i];
   }
   constexpr int OWN = Wave::NDT >= WK ? Wave::NDT / WK : 1;
@@ -908,7 +908,7 @@ __global__ __launch_bounds__(256, 1) void attn_window_few_kernel(AttnWindowParam
 #pragma unroll
     for (int i = 0; i < WK; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] += aw_rescaled(jb[((size_t)i * Wave::W + dt * 16 + e) * 64], f[i]);
+      for (int e = 0; e < 16; ++e) x[e] += jb[((size_t)i * Wave::W + dt * 16 + e) * 64] * f[i];
 #pragma unroll
     for (int a4 = 0; a4 < 4; ++a4)
       Wave::put(p, b, b.c0 + j, c.row, c.head, dt * 32 + 8 * a4 + 4 * h,
@@ -958,17 +958,17 @@ __global__ __launch_bounds__(256) void attn_window_finish(AttnWindowParams p, in
       float top = M;
 #pragma unroll
       for (int k = 0; k < 8; ++k) top = fmaxf(top, a[k].x);
-      const float keep = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - top);
+      const float keep = aw_rescale(M, top);
       M = top;
       l *= keep;
 #pragma unroll
-      for (int i = 0; i < E; ++i) o[i] = aw_rescaled(o[i], keep);
+      for (int i = 0; i < E; ++i) o[i] *= keep;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float f = a[k].x == -INFINITY ? 0.f : a[k].x == M ? 1.f : __builtin_amdgcn_exp2f(a[k].x - M);
+        const float f = aw_rescale(a[k].x, M);
         l += a[k].y * f;
 #pragma unroll
-        for (int i = 0; i < E; ++i) o[i] += aw_rescaled(x[k][i], f);
+        for (int i = 0; i < E; ++i) o[i] += x[k][i] * f;
       }
     }
     const float inv = 1.0f / l;
