@@ -221,7 +221,6 @@ struct SrLogits {
     head = min((int)((16 - ((uintptr_t)row & 15)) & 15) / (int)sizeof(T), vocab);
   }
   __device__ __forceinline__ float at(int i) const { return sr_clean((float)row[i]); }
-  __device__ __forceinline__ int begin(int c, int chunk) const { return c ? min(vocab, head + c * chunk) : 0; }
   __device__ __forceinline__ int end(int c, int chunk) const { return (int)min((long long)vocab, head + (c + 1ll) * chunk); }
   template <int THREADS, class F>
   __device__ __forceinline__ void each(int c, int chunk, F f) const {
