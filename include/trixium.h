@@ -223,8 +223,11 @@ int trx_gemv_packed_parts_f32(const uint8_t* packed, int kind, int M, int K, con
  * The ring holds the positions below pos that a query sees; slots that no visible position takes may
  * hold anything. Afterwards the new rows stand in their slots (of rows that share a slot, the last);
  * no other slot is written. An infinity or NaN in a key or value that a query does not see does not
- * reach its output; one in a value that it sees makes that element the same (inf and -inf: NaN). out,
+ * reach its output; one in a value that it sees makes that element the same (inf and -inf: NaN); one
+ * in the query or in a key that it sees may make the whole output row of that head NaN. out,
  * workspace and the ring overlap no other argument.
+ * Scores, maxima and sums are fp32. With TRX_KIND_F16 calls of many columns (n times the heads of a
+ * kv head; of a token or short turn never) also round each probability to fp16, by 2^-11 of itself.
  * pos_dev != NULL: the first position is read from the device when the work runs (for captured
  * graphs) and `pos` is ignored; a position there that is negative or leaves int32 within n leaves out
  * and the ring as they are.
@@ -260,7 +263,8 @@ int trx_attn_window(const trx_attn_window_shape* shape, int n, int pos, const in
  * kind: TRX_KIND_F32 or TRX_KIND_F16; row r at logits + r * ld (elements, ld >= vocab; any alignment
  * of the type's own). rows: device array of n settings (per_row), or one for every row. vocab <= 2^24,
  * n <= 2^20 (0: nothing is done). workspace: trx_sample_rows_geometry's bytes, 16-byte aligned, no
- * zeroing needed; calls that share it must not overlap. */
+ * zeroing needed; calls that share it must not overlap. top_k past 4096 together with top_p takes one
+ * block through the row some 15 times: 1.4 ms over 248320 logits, where either alone takes 36 us. */
 typedef struct trx_sampling {
   float temperature;
   int32_t top_k;

@@ -3,6 +3,8 @@
 `KVRing` holds the K and V rows of one layer on the GPU in the decoder's layout (fp16, position p in
 slot p below `pin`, else in a ring of the most recent positions; firmware/hybrid.c:156-181) and
 attends the next positions over them: any number at once (a prompt's chunk) or one (decoding).
+Queries, keys, values and outputs are numpy arrays, copied to the GPU and back by each call, which waits for
+it; a program whose data is on the GPU calls trx_attn_window with its own pointers, stream and workspace.
 """
 
 import ctypes

@@ -568,8 +568,8 @@ __device__ __forceinline__ uint32_t aw_tr(uint32_t tile, int lane) {
 // stage: behind it the rows that the stage before last read are replaced.
 // Bound by the matrix instructions and what of the vector and LDS work does not run beside them: a whole stage of
 // 128 dims with fp32 queries takes 3.3k cycles, of which 2.1k are matrix instructions (fp16: 2.2k and 1.0k); the
-// products reach 0.77 PFLOP/s over 1024 positions x 32 heads of 128 with a window of 2048 (two planes counted; the
-// launch 88 us), 0.70 over 1021 with a window of 6000 and fp16 queries (143 us). Eight waves, so that a SIMD has
+// products reach 0.80 PFLOP/s over 1024 positions x 32 heads of 128 with a window of 2048 (two planes counted; the
+// launch 86 us), 0.73 over 1021 with a window of 6000 and fp16 queries (139 us). Eight waves, so that a SIMD has
 // two (four of 256 dims: a wave's registers). Tried and slower: two tiles of columns a wave (200 against 139 us
 // then), two stages a barrier (equal), one of a SIMD's waves half a stage behind the other (98 against 90).
 // What is rare stands outside the loop, which the instruction cache then holds: 64 against 28 KB of code were
@@ -770,8 +770,8 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ * WK / 4) void attn_window_kernel(
 // keys at a time by itself, without barriers: its K rows come straight into the operand's registers, its V
 // rows through LDS of its own (to be read transposed), both one tile ahead; the queries, the same for
 // all four, lie in LDS to leave the registers to the rows. Bound by the rows' latency and
-// bytes, the joins and, for short windows, the two launches: one position over 32768 keys (134 MB) 25 us, 5.4 TB/s,
-// and 6 in the second launch; over 1024 keys (4.2 MB) 9 and 3.
+// bytes, the joins and, for short windows, the two launches: one position over 32768 keys (134 MB) 26 us, 5.3 TB/s,
+// and 6 in the second launch; over 1024 keys (4.2 MB) 10 and 3.
 template <int HD, bool HALF>
 __global__ __launch_bounds__(256, 1) void attn_window_few_kernel(AttnWindowParams p) {
   using Wave = AwWave<HD, HALF, true>;

@@ -14,13 +14,16 @@
 // No sort of the vocabulary: a histogram over 1024 steps of the logit's distance from the largest
 // (counts and masses) finds the step that the cut falls into; the tokens of that step, or with a short
 // list every token up to it, are gathered, and the cut is found among them by nine bits of (logit,
-// index) at a time. A row whose cut step holds more than a block gathers (many equal or nearly equal
-// logits) is cut by the same rounds over the row itself.
+// index) at a time. A row is cut by one block, by the same rounds over the row itself (two rounds of the search with
+// both filters, each some seven readings), where its cut step holds more than a row's gather (many equal or nearly
+// equal logits) or tokens without mass, and where top_k and top_p are both set and the tokens up to top_k's step are
+// more than that: what top_p asks for is not known before top_k's cut is. That is slow: top_k 5000 with top_p over
+// 248320 logits 1406 us for one row, 1442 for 24, 1684 for 160; with top_k alone 36, 69, 187, with top_p alone 34, 81, 200.
 //
 // What bounds it: many rows, reading them (the largest logits, the histogram, the gather; for a row drawn from more
 // than was gathered, the masses) and the 64-bit exponentials; a single row, six launches that wait for each other.
-// us per launch, 160 rows of 248320 fp32 logits (159 MB) with top_p: 28 (5.7 TB/s), 61 (without the
-// exponentials 42), 39, the cuts 20, masses 20, draws 9; one row of 151936: 4, 7, 7, 4, 2, 1.
+// us per launch, 160 rows of 248320 fp32 logits (159 MB) with top_p: 28 (5.7 TB/s), 59 (without the
+// exponentials 42), 38, the cuts 20, masses 20, draws 9; one row of 151936: 4, 7, 7, 4, 2, 1.
 
 #include "trx_sample.h"
 

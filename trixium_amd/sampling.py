@@ -1,6 +1,8 @@
 """Sampling one token per row of logits from the whole vocabulary (host side of trx_sample_rows):
 temperature, top-k, top-p and min-p, from given uniform numbers. The firmware's own sampler, which
-draws among 32 candidates, is `Decoder.set_sampling` (firmware/infer.c:385-488)."""
+draws among 32 candidates, is `Decoder.set_sampling` (firmware/infer.c:385-488). Logits and results are
+numpy arrays, copied to the GPU and back by each call, which waits for it; a program whose logits are on the GPU
+calls trx_sample_rows with its own pointers, stream and workspace, and the decoder does (set_vocab_sampling)."""
 
 import ctypes
 
