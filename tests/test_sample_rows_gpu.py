@@ -162,6 +162,16 @@ def test_a_top_k_past_int32_is_off(monkeypatch):
     assert seen[:4] == [2**31 - 1, -1, 40, 0]
 
 
+@pytest.mark.parametrize("dtype", [np.uint8, np.int8, np.uint16, np.int16, np.uint32, np.int64, np.uint64, np.float16,
+                                   np.float64, bool, object])
+def test_settings_take_a_top_k_of_any_type(dtype):
+    assert settings(top_k=np.array([1, 0], dtype))["top_k"].tolist() == [1, 0]
+    if dtype in (np.uint32, np.int64, np.uint64, np.float64, object):
+        assert settings(top_k=np.array([2**32 - 1, 50], dtype))["top_k"].tolist() == [2**31 - 1, 50]
+    if dtype is object:
+        assert settings(top_k=np.array([2**70], dtype))["top_k"].tolist() == [2**31 - 1]
+
+
 # Results (GPU) ---------------------------------------------------------------------------------------
 
 

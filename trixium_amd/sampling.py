@@ -17,7 +17,8 @@ ROW = np.dtype([("temperature", np.float32), ("top_k", np.int32), ("top_p", np.f
 def settings(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """One row's settings (scalars), or n rows' (arrays of n or scalars), as trx_sampling structs. top_k 0,
     top_p 1 and min_p 0 are off; temperature 0 takes the largest logit."""
-    top_k = np.clip(top_k, -1, 2**31 - 1)          # (past int32: off, like every one past the vocabulary)
+    top_k = np.asarray(top_k)                      # (past int32: off, like every one past the vocabulary)
+    top_k = np.clip(top_k.astype(np.int64 if top_k.dtype.kind in "bui" else np.float64), -1, 2**31 - 1)
     cols = np.broadcast_arrays(*(np.atleast_1d(a) for a in (temperature, top_k, top_p, min_p)))
     out = np.empty(cols[0].shape, dtype=ROW)
     for name, c in zip(ROW.names, cols):
