@@ -622,3 +622,11 @@ def test_repeated_calls_give_the_same_bits(kind, heads, kv, hd, window, n):
     for _ in range(4):
         for a, b in zip(first, _call(c, q, k, v, first[1], first[2], pos=2 * window)):
             assert np.array_equal(a.view(np.uint8), b.view(np.uint8))
+
+
+@pytest.mark.parametrize("change", [dict(window=2**32 + 10), dict(sinks=2**32 + 1), dict(pin=2**32 + 4, sinks=4, window=60),
+                                    dict(slots=2**32 + 64, window=60), dict(n_head=2**32 + 4), dict(head_dim=2**32 + 64)])
+def test_kv_ring_refuses_what_int32_does_not_hold(change):
+    from trixium_amd.attention import KVRing
+    with pytest.raises(ValueError):
+        KVRing(**{**dict(n_head=4, n_kv_head=2, head_dim=64, slots=64, pin=4), **change})

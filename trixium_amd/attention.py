@@ -31,11 +31,14 @@ class KVRing:
         self.n_head, self.n_kv, self.hd, self.slots = int(n_head), int(n_kv_head), int(head_dim), int(slots)
         self.dtype = _DTYPES[kind]
         q, kv = self.n_head * self.hd, self.n_kv * self.hd
-        self.shape = _lib.AttnWindowShape(
+        shape = dict(
             kind=kind, n_head=self.n_head, n_kv_head=self.n_kv, head_dim=self.hd, slots=self.slots, pin=int(pin),
             window=int(self.slots - pin if window is None else window), sinks=int(pin if sinks is None else sinks),
-            q_stride=q, kv_stride=kv, out_stride=q, gate_stride=q, gate_head_stride=self.hd,
-            scale=1.0 / math.sqrt(self.hd) if scale is None else scale)
+            q_stride=q, kv_stride=kv, out_stride=q, gate_stride=q, gate_head_stride=self.hd)
+        for name, v in shape.items():              # (ctypes would take them modulo 2^32)
+            if not -2**31 <= v < 2**31:
+                raise ValueError(f"{name} {v} is not an int32")
+        self.shape = _lib.AttnWindowShape(scale=1.0 / math.sqrt(self.hd) if scale is None else scale, **shape)
         self.work, self.work_n = None, 0           # the workspace, of calls of up to work_n positions
         self._workspace(1)                         # refuses an unsupported shape before any allocation
         self.position = 0                          # of the next row
