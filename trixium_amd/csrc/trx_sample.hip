@@ -14,8 +14,8 @@
 // No sort of the vocabulary: a histogram over 1024 steps of the logit's distance from the largest
 // (counts and masses) finds the step that the cut falls into; the tokens of that step, or with a short
 // list every token up to it, are gathered, and the cut is found among them by nine bits of (logit,
-// index) at a time. A row is cut by one block, by the same rounds over the row itself (two rounds of the search with
-// both filters, each some seven readings), where its cut step holds more than a row's gather (many equal or nearly
+// index) at a time. A row is cut by one block, by the same rounds over the row itself (some seven readings a filter,
+// twice that with both), where its cut step holds more than a row's gather (many equal or nearly
 // equal logits) or tokens without mass, and where top_k and top_p are both set and the tokens up to top_k's step are
 // more than that: what top_p asks for is not known before top_k's cut is. That is slow: top_k 5000 with top_p over
 // 248320 logits 1406 us for one row, 1442 for 24, 1684 for 160; with top_k alone 36, 69, 187, with top_p alone 34, 81, 200.
