@@ -245,6 +245,86 @@ int trx_attn_window(const trx_attn_window_shape* shape, int n, int pos, const in
                     const uint16_t* k, const uint16_t* v, uint16_t* kcache, uint16_t* vcache,
                     const void* gate, void* out, void* workspace, trx_stream_t s);
 
+/* Drafts behind a shared prefix --------------------------------------------------------------------
+ * Attention of the next positions of `batch` drafts (sequences) that share a prefix, whose rows of K and V
+ * stand once for all: fp16 [n_kv_head][prefix_slots][head_dim], the decoder's layout, of which the first
+ * `prefix` rows count. Each draft has a tail of its own, fp16 [batch][n_kv_head][tail_slots][head_dim], with
+ * lengths[b] rows. Rows b * n .. b * n + n - 1 of q, k, v, gate and out are draft b's next ones, of which the
+ * first counts[b] count (counts NULL: all n). New row i of draft b sees the prefix, the draft's tail and its
+ * new rows 0 .. i:
+ *   out = sum e^(scale q.k_u) v_u / sum e^(scale q.k_u), times sigmoid(gate) with gate != NULL
+ * (model/fastref.py:31-43 attention_fp32, :216-241). Afterwards the new rows stand in slots lengths[b] ..
+ * of the draft's tail; the caller moves lengths on. No counterpart in the reference, which decodes one sequence.
+ * lengths and counts are read from the device when the work runs (a captured call follows them). A draft whose
+ * count is not in [1, n], or whose length is negative or leaves tail_slots within its count, takes no part: its
+ * rows of out and its tail stay as they are, as do the rows of out behind a draft's count; their q, k, v and
+ * gate may hold anything.
+ * kind, head sizes, row strides, alignment and the treatment of infinities and NaN are trx_attn_window's;
+ * lengths and counts are 4-byte aligned. prefix <= prefix_slots <= 2^30 (0: kprefix and vprefix may be NULL),
+ * 1 <= tail_slots <= 2^30, batch * n * n_head <= 2^23 (batch or n 0: nothing is done). out, workspace and the
+ * tails overlap no other argument.
+ * workspace: trx_attn_shared_geometry's bytes, which hold any call of the shape of up to `batch` drafts, `n` new
+ * rows and any prefix, no zeroing needed; calls that share it must not overlap. */
+typedef struct trx_attn_shared_shape {
+  int kind;
+  int n_head, n_kv_head, head_dim;
+  int prefix_slots, tail_slots;
+  int q_stride, kv_stride, out_stride, gate_stride, gate_head_stride;
+  float scale;
+} trx_attn_shared_shape;
+int trx_attn_shared_geometry(const trx_attn_shared_shape* shape, int batch, int n, int prefix, size_t* workspace_bytes);
+int trx_attn_shared(const trx_attn_shared_shape* shape, int batch, int n, int prefix, const int32_t* lengths,
+                    const int32_t* counts, const void* q, const uint16_t* k, const uint16_t* v,
+                    const uint16_t* kprefix, const uint16_t* vprefix, uint16_t* ktail, uint16_t* vtail,
+                    const void* gate, void* out, void* workspace, trx_stream_t s);
+
+/* A cache that knows its rows' weight, and eviction by it ----------------------------------------------
+ * The cache of one sequence: `slots` rows per kv head of K and V (fp16 [n_kv_head][slots][head_dim], the
+ * decoder's layout), of masses (fp32 [n_kv_head][slots]) and of positions (int32 [n_kv_head][slots]). The
+ * first `count` slots of every kv head hold rows; which positions they are may differ from head to head.
+ *
+ * trx_attn_mass: attention of the next n positions pos .. pos + n - 1 over the cache. New row i sees the `count`
+ * rows and the new rows 0 .. i (out as for trx_attn_shared), and gives every row that it sees the probability
+ * that it has for it: mass[g][u] += the sum over the new rows and the heads of kv head g of
+ * e^(scale q.k_u) / sum e^(scale q.k_u'); the masses of the new rows begin with this call's. The new rows, their
+ * masses and positions take slots count .. count + n - 1; the caller moves count on. No other slot is written but
+ * for the masses of the first `count`. count + n <= slots.
+ * state != NULL: {count, pos} are read from the device when the work runs (for captured graphs) and the
+ * arguments ignored; values out of range there leave everything as it is.
+ * kind, head sizes, row strides, alignment and the treatment of infinities and NaN are trx_attn_window's; mass,
+ * positions and state are 4-byte aligned. An infinity or NaN in the query or in a key that it sees may also make
+ * the masses of its kv head NaN. slots <= 2^30, n * n_head <= 2^23 (n = 0: nothing is done).
+ * Masses do not depend on the order of blocks: the same call gives the same bits.
+ * workspace: trx_attn_mass_geometry's bytes for n, which hold any call of the shape of up to n positions, no
+ * zeroing needed; calls that share it must not overlap.
+ *
+ * trx_kv_evict: of the `count` rows of every kv head, `keep` stay: those at positions below `sinks` or from
+ * pos - recent on (pos: the next row's position) before any other, then those of the largest masses (a NaN is
+ * below every number), equal ones by slot. Of what stays, the rows from slot `keep` on take the slots below it of
+ * rows that go, first to first; K, V, mass and position of a row move together. The cache then holds `keep` rows;
+ * nothing else is written. keep >= count: nothing is done. 1 <= keep <= slots, 0 <= count <= slots, sinks >= 0,
+ * recent >= 0, pos >= 0. Of the shape the heads, head_dim and slots count.
+ * state != NULL: {count, pos} from the device, as above.
+ * Rows do not stand in the order of their positions afterwards; attention does not ask for it. Each row's bits
+ * are what they were.
+ * workspace: trx_kv_evict_geometry's bytes, 16-byte aligned, no zeroing needed; calls that share it must not
+ * overlap. No counterpart of either in the reference, whose ring drops the oldest position. */
+typedef struct trx_attn_mass_shape {
+  int kind;
+  int n_head, n_kv_head, head_dim;
+  int slots;
+  int q_stride, kv_stride, out_stride, gate_stride, gate_head_stride;
+  float scale;
+} trx_attn_mass_shape;
+int trx_attn_mass_geometry(const trx_attn_mass_shape* shape, int n, size_t* workspace_bytes);
+int trx_attn_mass(const trx_attn_mass_shape* shape, int n, int count, int pos, const int32_t* state, const void* q,
+                  const uint16_t* k, const uint16_t* v, uint16_t* kcache, uint16_t* vcache, float* mass,
+                  int32_t* positions, const void* gate, void* out, void* workspace, trx_stream_t s);
+int trx_kv_evict_geometry(const trx_attn_mass_shape* shape, size_t* workspace_bytes);
+int trx_kv_evict(const trx_attn_mass_shape* shape, int count, int pos, const int32_t* state, int keep, int sinks,
+                 int recent, uint16_t* kcache, uint16_t* vcache, float* mass, int32_t* positions, void* workspace,
+                 trx_stream_t s);
+
 /* Sampling from the whole vocabulary --------------------------------------------------------------
  * One token per row of logits by temperature, top-k, top-p and min-p from a given uniform number (the
  * firmware's sampler, firmware/infer.c:385-488, draws among 32 candidates; trx_model_set_sampling).

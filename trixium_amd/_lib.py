@@ -55,6 +55,19 @@ class AttnWindowShape(ctypes.Structure):
                                             "gate_head_stride")] + [("scale", ctypes.c_float)]
 
 
+class AttnSharedShape(ctypes.Structure):
+    """trx_attn_shared_shape (include/trixium.h): heads, slots and strides of drafts behind a shared prefix."""
+    _fields_ = [(n, ctypes.c_int) for n in ("kind", "n_head", "n_kv_head", "head_dim", "prefix_slots", "tail_slots",
+                                            "q_stride", "kv_stride", "out_stride", "gate_stride",
+                                            "gate_head_stride")] + [("scale", ctypes.c_float)]
+
+
+class AttnMassShape(ctypes.Structure):
+    """trx_attn_mass_shape (include/trixium.h): heads, slots and strides of a cache with masses."""
+    _fields_ = [(n, ctypes.c_int) for n in ("kind", "n_head", "n_kv_head", "head_dim", "slots", "q_stride", "kv_stride",
+                                            "out_stride", "gate_stride", "gate_head_stride")] + [("scale", ctypes.c_float)]
+
+
 SIGNATURES = {
     "trx_last_error": [],
     "trx_version": [],
@@ -92,6 +105,12 @@ SIGNATURES = {
     "trx_gemv_set_variant": [_i],
     "trx_attn_window_geometry": [ctypes.POINTER(AttnWindowShape), _i, ctypes.POINTER(_sz)],
     "trx_attn_window": [ctypes.POINTER(AttnWindowShape), _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "trx_attn_shared_geometry": [ctypes.POINTER(AttnSharedShape), _i, _i, _i, ctypes.POINTER(_sz)],
+    "trx_attn_shared": [ctypes.POINTER(AttnSharedShape), _i, _i, _i] + [_vp] * 13,
+    "trx_attn_mass_geometry": [ctypes.POINTER(AttnMassShape), _i, ctypes.POINTER(_sz)],
+    "trx_attn_mass": [ctypes.POINTER(AttnMassShape), _i, _i, _i] + [_vp] * 12,
+    "trx_kv_evict_geometry": [ctypes.POINTER(AttnMassShape), ctypes.POINTER(_sz)],
+    "trx_kv_evict": [ctypes.POINTER(AttnMassShape), _i, _i, _vp, _i, _i, _i] + [_vp] * 6,
     "trx_sample_rows_geometry": [_i, _i, ctypes.POINTER(_sz)],
     "trx_sample_rows": [_vp, _i, _i, _i, ctypes.c_int64, _vp, _i, _vp, _vp, _vp, _vp, _vp],
     "trx_model_create": [_mcp, _fp, ctypes.POINTER(_vp)],

@@ -1,0 +1,537 @@
+// Attention over caches whose rows stand one behind the other, on the tiles of trx_attn_tile.h:
+// - drafts behind a shared prefix: o = sum_u e^{scale q.k_u - m} v_u / sum_u e^{scale q.k_u - m} over the prefix's
+//   rows, the draft's tail and its new rows up to the query's own. The sum splits at the prefix's end: the
+//   prefix takes the columns of all drafts together, so that its rows are read once for all of them, a tail those
+//   of its draft; the parts (m, the sum behind m, the outputs) are joined by the second launch.
+// - one sequence with masses: mass_u += sum of e^{scale q.k_u - m} / sum_u' e^{scale q.k_u' - m} over the positions
+//   and heads of the kv head. The final sums have to be there: calls of few columns keep their scores (a column's
+//   4 bytes a key, beside the key's 4 hd bytes of K and V) and the second launch adds their probabilities up; of
+//   many columns the scores are taken again, keys staying where the columns pass.
+// No sum depends on the order of blocks.
+
+#include "trx_attn_rows.h"
+#include "trx_attn_tile.h"
+
+#include <algorithm>
+#include <limits.h>
+
+namespace trx {
+
+// The rows that sequence seq has and gets; whether it takes part.
+__device__ __forceinline__ bool ar_sequence(const AttnRowsParams& p, int seq, int& have, int& fresh) {
+  have = p.state ? p.state[0] : p.lengths ? p.lengths[seq] : p.length;
+  fresh = p.counts ? p.counts[seq] : p.n;
+  return have >= 0 && fresh > 0 && fresh <= p.n && have <= p.tail_slots - fresh;
+}
+__device__ __forceinline__ bool ar_position(const AttnRowsParams& p, int& pos) {
+  pos = p.state ? p.state[1] : p.pos;
+  return pos >= 0 && pos <= INT_MAX - p.n;
+}
+
+// A probability is 2^(score - norm.x) norm.y: of a column's reference and the sum behind it.
+__device__ __forceinline__ float2 ar_norm(float M, float l) { return make_float2(M - kAwBias, 1.f / l); }
+
+// What the waves of a block know of their work. Keys x below `cached` stand in the cache, the others are new rows.
+struct ArBlock {
+  int g, sp, c0, end;          // kv head; part; first column and that behind the last
+  int split, splits;           // of the keys
+  int N, cached, row0, seq;    // keys; the draft's first row
+  bool tail;
+};
+
+// The column of a lane (32 a wave, lanes j and j + 32 the same): it sees the keys below lim.
+struct ArColumn {
+  int row, head, lim, w_first; // w_first: the smallest limit of the wave's columns
+
+  __device__ __forceinline__ ArColumn(const AttnRowsParams& p, const ArBlock& b, int first, int j) {
+    const int last = b.end - 1, col = min(first + j, last);
+    row = aw_row(p, col);
+    head = b.g * p.rep + (col - row * p.rep);
+    lim = b.tail ? b.cached + row - b.row0 + 1 : b.N;
+    w_first = b.tail ? b.cached + aw_row(p, min(first, last)) - b.row0 + 1 : b.N;
+  }
+};
+
+template <int HD>
+struct ArRows {
+  const char *kc, *vc;         // the cache's rows of the kv head
+  long long kd, vd;            // from there to the call's own rows
+  int kv_stride;
+
+  __device__ __forceinline__ ArRows(const AttnRowsParams& p, const ArBlock& b) : kv_stride(p.kv_stride) {
+    const size_t at = b.tail ? ((size_t)b.seq * p.n_kv + b.g) * p.tail_slots * HD : (size_t)b.g * p.prefix_slots * HD;
+    kc = (const char*)((b.tail ? (const __half*)p.ktail : p.kprefix) + at);
+    vc = (const char*)((b.tail ? (const __half*)p.vtail : p.vprefix) + at);
+    const size_t own = (size_t)b.row0 * p.kv_stride + (size_t)b.g * HD;
+    kd = (const char*)(p.k + own) - kc;
+    vd = (const char*)(p.v + own) - vc;
+  }
+  // Byte distance of key x's row from the cache's rows (past the last key: that key again, masked), and all ones
+  // if it is one of the call's own.
+  __device__ __forceinline__ long long row(const ArBlock& b, int x, long long& fresh) const {
+    x = min(x, b.N - 1);
+    const bool own = x >= b.cached;
+    fresh = own ? -1 : 0;
+    return 2ll * (own ? x - b.cached : x) * (own ? kv_stride : HD);
+  }
+  // How many runs of `count` keys from key x0 on lie evenly spaced (uniform); with one at least, the first
+  // one's distance and the step in bytes.
+  __device__ __forceinline__ int flat(const ArBlock& b, int x0, int count, long long& at, bool& own, uint32_t& step) const {
+    if (x0 >= b.N) return 0;
+    own = x0 >= b.cached;
+    step = 2u * (uint32_t)(own ? kv_stride : HD);
+    at = own ? 2ll * (x0 - b.cached) * kv_stride : 2ll * x0 * HD;
+    return ((own ? b.N : b.cached) - x0) / count;
+  }
+};
+
+// Rows in a line as a layout of the keys (trx_attn_tile.h).
+template <int HD, bool MASS>
+struct ArLine {
+  using Params = AttnRowsParams;
+  using Block = ArBlock;
+  using Rows = ArRows<HD>;
+  using Column = ArColumn;
+
+  // A kv head's blocks stay on the XCDs of its number (blocks go round-robin over them), so that the prefix and a
+  // sequence's rows are read into few L2s.
+  __device__ __forceinline__ static bool block(const Params& p, int columns, Block& b) {
+    unsigned i = blockIdx.x, t;
+    b.tail = i >= (unsigned)p.prefix_blocks;
+    if (!b.tail) {
+      t = i / (unsigned)p.n_kv;
+      b.g = (int)(i - t * p.n_kv);
+      b.splits = p.prefix_splits;
+      b.split = b.sp = (int)(t / (unsigned)p.prefix_cb);
+      b.c0 = (int)(t - (unsigned)b.split * p.prefix_cb) * columns;
+      b.end = p.cols;
+      b.seq = b.row0 = 0;
+      b.N = b.cached = p.prefix;
+      return true;
+    }
+    i -= p.prefix_blocks;
+    t = i / (unsigned)p.n_kv;
+    b.g = (int)(i - t * p.n_kv);
+    i = t / (unsigned)p.tail_splits;
+    b.splits = p.tail_splits;
+    b.split = (int)(t - i * p.tail_splits);
+    b.sp = p.prefix_splits + b.split;
+    b.seq = (int)(i / (unsigned)p.tail_cb);
+    const int cb = (int)(i - (unsigned)b.seq * p.tail_cb);
+    int fresh, pos;
+    if (!ar_sequence(p, b.seq, b.cached, fresh) || (MASS && !ar_position(p, pos))) return false;
+    b.row0 = b.seq * p.n;
+    b.c0 = b.row0 * p.rep + cb * columns;
+    b.end = (b.row0 + fresh) * p.rep;
+    if (b.c0 >= b.end) return false;
+    b.N = b.cached + aw_row(p, min(b.c0 + columns, b.end) - 1) - b.row0 + 1;
+    return true;
+  }
+  // Whether the column sees key x.
+  __device__ __forceinline__ static auto sight(const Params&, const Block&, const Column& c) {
+    return [lim = c.lim](int x) AW_INLINE { return x < lim; };
+  }
+  // Whole stages are [a0, a1) of those whose wave takes keys SR st + own .. + 31.
+  __device__ __forceinline__ static void whole(const Params&, const Block&, const Column& c, int own, int SR, int& a0, int& a1) {
+    a0 = 0;
+    a1 = c.w_first - kAwKeys < own ? 0 : (c.w_first - kAwKeys - own) / SR + 1;
+  }
+  __device__ __forceinline__ static bool all_see(const Params&, const Block&, const Column& c, int x0) {
+    return x0 + kAwKeys <= c.w_first;
+  }
+  // A lane's scores of keys x, x + 8, x + 16 and x + 24, four each, in powers of two.
+  __device__ __forceinline__ static void scored(const Params& p, const Block& b, int col, int x, const f32x16_t& s, float cs) {
+    if (MASS && p.scores) {
+      float* to = p.scores + ((size_t)b.g * p.cols + col) * p.score_ld + x;
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+        *(float4*)(to + 8 * a) = make_float4(s[4 * a] * cs, s[4 * a + 1] * cs, s[4 * a + 2] * cs, s[4 * a + 3] * cs);
+    }
+  }
+  __device__ __forceinline__ static void total(const Params& p, const Block& b, int col, const float2& ml) {
+    if constexpr (MASS) p.norms[(size_t)b.g * p.cols + col] = ar_norm(ml.x, ml.y);
+  }
+};
+
+template <int HD, bool HALF, bool MASS, int WQ, int WK, int D>
+__global__ __launch_bounds__(64 * WQ * WK, WQ * WK / 4) void attn_rows_kernel(AttnRowsParams p) {
+  aw_many<ArLine<HD, MASS>, HD, HALF, WQ, WK, D>(p);
+}
+
+template <int HD, bool HALF, bool MASS>
+__global__ __launch_bounds__(256, 1) void attn_rows_few_kernel(AttnRowsParams p) {
+  aw_few<ArLine<HD, MASS>, HD, HALF>(p);
+}
+
+// Few columns: one more key's mass a thread, from the scores that the attention kept. The columns' parts are joined
+// anew by every block: 32 columns, 8 lanes each.
+__device__ __forceinline__ void ar_mass_few(const AttnRowsParams& p, int block, float2* norm) {
+  int have, fresh;
+  if (!ar_sequence(p, 0, have, fresh)) return;
+  const int kb = block / p.n_kv, g = block - kb * p.n_kv, x = kb * 256 + threadIdx.x, N = have + fresh;
+  if (kb * 256 >= N) return;
+  const int c = threadIdx.x >> 3;
+  float M = -INFINITY, l = 0.f;
+  if (p.nsplit > 1) {
+    const size_t all = (size_t)p.nsplit * p.n_kv * p.cols;
+    const float2* ml = (const float2*)((const float*)p.work + all * p.hd) + (size_t)g * p.cols + c;
+    for (int s = threadIdx.x & 7; s < p.nsplit && c < p.cols; s += 8) {
+      const float2 a = ml[(size_t)s * p.n_kv * p.cols];
+      const float to = fmaxf(M, a.x);
+      l = l * aw_rescale(M, to) + a.y * aw_rescale(a.x, to);
+      M = to;
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+      const float m1 = __shfl_xor(M, o, 64), l1 = __shfl_xor(l, o, 64), to = fmaxf(M, m1);
+      l = l * aw_rescale(M, to) + l1 * aw_rescale(m1, to);
+      M = to;
+    }
+    if ((threadIdx.x & 7) == 0) norm[c] = ar_norm(M, l);
+  } else if ((threadIdx.x & 7) == 0 && c < p.cols) {
+    norm[c] = p.norms[(size_t)g * p.cols + c];
+  }
+  __syncthreads();
+  if (x >= N) return;
+  const float* s = p.scores + (size_t)g * p.cols * p.score_ld + x;
+  float sum = 0.f;
+  for (int i = 0; i < p.cols; ++i) sum = fmaf(__builtin_amdgcn_exp2f(s[i * p.score_ld] - norm[i].x), norm[i].y, sum);
+  float* m = p.mass + (size_t)g * p.tail_slots + x;
+  *m = x < have ? *m + sum : sum;
+}
+
+// After the attention: the parts of each (row, head) joined (a wave each, blocks of four), the new rows into the
+// tails' slots, and the masses of calls of few columns.
+template <int HD, bool HALF, bool MASS>
+__global__ __launch_bounds__(256) void attn_rows_finish(AttnRowsParams p, int join_blocks, int append_blocks) {
+  __shared__ float2 norm[32];
+  int pos = 0;
+  if (MASS && !ar_position(p, pos)) return;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  if ((int)blockIdx.x < join_blocks) {
+    const unsigned id = blockIdx.x * 4 + w;         // below 2^23 + 4
+    if (id >= (unsigned)(p.batch * p.n * p.n_head)) return;
+    const int row = (int)(id / (unsigned)p.n_head), head = (int)id - row * p.n_head, seq = row / p.n;
+    int have, fresh;
+    if (!ar_sequence(p, seq, have, fresh) || row - seq * p.n >= fresh) return;
+    float M, l;
+    aw_join<HD, HALF>(p, row, head, lane, M, l);
+    if (MASS && lane == 0) {
+      const int g = aw_row(p, head);
+      p.norms[(size_t)g * p.cols + row * p.rep + head - g * p.rep] = ar_norm(M, l);
+    }
+    return;
+  }
+  if ((int)blockIdx.x < join_blocks + append_blocks) {
+    // 16 bytes of K and V a thread.
+    constexpr int SEG = HD / 8;
+    const long long id = (long long)(blockIdx.x - join_blocks) * 256 + threadIdx.x;
+    if (id >= (long long)p.batch * p.n * p.n_kv * SEG) return;
+    const unsigned at = (unsigned)(id / SEG);        // below 2^23
+    const int sd = (int)(id % SEG) * 8, row = (int)(at / (unsigned)p.n_kv), g = (int)at - row * p.n_kv, seq = row / p.n;
+    const int i = row - seq * p.n;
+    int have, fresh;
+    if (!ar_sequence(p, seq, have, fresh) || i >= fresh) return;
+    const size_t slot = ((size_t)seq * p.n_kv + g) * p.tail_slots + have + i;
+    const size_t from = (size_t)row * p.kv_stride + (size_t)g * HD + sd;
+    *(uint4*)(p.ktail + slot * HD + sd) = *(const uint4*)(p.k + from);
+    *(uint4*)(p.vtail + slot * HD + sd) = *(const uint4*)(p.v + from);
+    if (MASS && sd == 0) p.positions[slot] = pos + i;
+    return;
+  }
+  if constexpr (MASS) ar_mass_few(p, blockIdx.x - join_blocks - append_blocks, norm);
+}
+
+// Many columns: the masses of 32 keys a wave, which holds the keys' rows while the columns pass, 32 at a time.
+template <int HD, bool HALF>
+__global__ __launch_bounds__(256) void attn_mass_kernel(AttnRowsParams p) {
+  using Wave = AwWave<ArLine<HD, true>, HD, HALF, false>;
+  const int kb = blockIdx.x / (unsigned)p.n_kv, w = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 5, j = lane & 31;
+  ArBlock b;
+  int pos, fresh;
+  b.g = (int)blockIdx.x - kb * p.n_kv;
+  b.seq = b.row0 = 0;
+  b.tail = true;
+  if (!ar_sequence(p, 0, b.cached, fresh) || !ar_position(p, pos)) return;
+  b.N = b.cached + fresh;
+  const int x0 = (kb * 4 + w) * kAwKeys;
+  if (x0 >= b.N) return;
+  const ArRows<HD> rows(p, b);
+  long long own;
+  const long long at = rows.row(b, x0 + j, own);
+  const char* kr = rows.kc + at + (rows.kd & own) + 16 * h;
+  half8_t kf[Wave::NC];
+#pragma unroll
+  for (int k = 0; k < Wave::NC; ++k) kf[k] = *(const half8_t*)(kr + 32 * k);
+  f32x16_t sum = {};
+  // Columns before the first new row that sees key x0 have nothing for the tile.
+  for (int c0 = max(0, x0 - b.cached) * p.rep; c0 < p.cols; c0 += 32) {
+    const int col = min(c0 + j, p.cols - 1), row = aw_row(p, col), head = b.g * p.rep + col - row * p.rep;
+    const char* qr = (const char*)p.q + ((size_t)row * p.q_stride + (size_t)head * HD) * (HALF ? 2 : 4);
+    AwQuery<HD, HALF> q;
+    const float cs = q.take(p.scale, h, [&](int i) { return *(const u32x4_t*)(qr + 16 * i); });
+    const float2 norm = p.norms[(size_t)b.g * p.cols + col];
+    const f32x16_t s = Wave::scores([&](int k) { return kf[k]; }, [&](int k) { return q.hi[k]; },
+                                    [&](int k) { return q.lo[HALF ? 0 : k]; });
+    const int lim = c0 + j < p.cols ? b.cached + row + 1 : 0;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int x = x0 + 8 * (e >> 2) + 4 * h + (e & 3);
+      sum[e] = x < lim ? fmaf(__builtin_amdgcn_exp2f(fmaf(s[e], cs, -norm.x)), norm.y, sum[e]) : sum[e];
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sum[e] += __shfl_xor(sum[e], o, 64);
+  if (j) return;
+  float* m = p.mass + (size_t)b.g * p.tail_slots;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const int x = x0 + 8 * (e >> 2) + 4 * h + (e & 3);
+    if (x < b.N) m[x] = x < b.cached ? m[x] + sum[e] : sum[e];
+  }
+}
+
+// Launch ------------------------------------------------------------------------------------------
+
+constexpr int kArBlocks = 512;                      // blocks that a cut of the keys aims at
+constexpr int kArMaxPrefixSplits = 64, kArMaxTailSplits = 16;
+
+// How a call is cut: splits of the prefix's and of the tails' keys, in column blocks of 32.
+struct ArPlan {
+  int prefix, tail;
+};
+static int ar_splits(long long blocks, int keys, int most) {
+  const int tiles = cdiv(keys, kAwKeys);
+  return (int)std::max(1ll, std::min({(long long)most, kArBlocks / std::max(blocks, 1ll), (long long)tiles / 4}));
+}
+// The rows that a tail has at most after the call.
+static int ar_most_rows(const AttnRowsParams& p) { return p.state || p.lengths ? p.tail_slots : p.length + p.n; }
+static ArPlan ar_plan(const AttnRowsParams& p) {
+  const int rep = p.n_head / p.n_kv;
+  const long long prefix = (long long)cdiv(p.batch * p.n * rep, 32) * p.n_kv, tail = (long long)p.batch * cdiv(p.n * rep, 32) * p.n_kv;
+  return {p.prefix > 0 ? ar_splits(prefix, p.prefix, kArMaxPrefixSplits) : 0, ar_splits(tail, ar_most_rows(p), kArMaxTailSplits)};
+}
+
+const char* attn_rows_refuses(const AttnRowsParams& p) {
+  if (p.hd != 64 && p.hd != 128 && p.hd != 256) return "head_dim is not 64, 128 or 256";
+  if (p.n_kv < 1 || p.n_head < 1 || p.n_head % p.n_kv) return "n_head is not a multiple of n_kv_head";
+  if (p.n_head > 1024) return "more than 1024 heads";
+  if (p.prefix_slots < 0 || p.prefix_slots > 1 << 30 || p.tail_slots < 1 || p.tail_slots > 1 << 30) return "slots outside [1, 2^30]";
+  if (p.prefix < 0 || p.prefix > p.prefix_slots) return "prefix outside [0, prefix_slots]";
+  // (Blocks of 256 threads, one a column at most, stay below a grid's 2^32 threads.)
+  if (p.batch < 0 || p.n < 0 || (p.batch > 0 && (long long)p.n * p.n_head > (1 << 23) / p.batch)) return "too many rows";
+  if (!(p.scale > 0.f && p.scale < INFINITY)) return "scale is not positive and finite";
+  const int q4 = p.half_io ? 8 : 4, o4 = 4;
+  if (p.q_stride < p.n_head * p.hd || p.q_stride % q4) return "q_stride";
+  if (p.kv_stride < p.n_kv * p.hd || p.kv_stride % 8 || p.kv_stride > 1 << 22) return "kv_stride";
+  if (p.out_stride < p.n_head * p.hd || p.out_stride % o4) return "out_stride";
+  if (p.gate && (p.gate_head_stride < p.hd || p.gate_head_stride % o4 || p.gate_stride % o4 ||
+                 p.gate_stride < (long long)(p.n_head - 1) * p.gate_head_stride + p.hd))
+    return "gate strides";
+  return nullptr;
+}
+
+static long long ar_score_ld(const AttnRowsParams& p) { return ((long long)p.tail_slots + 31) / 32 * 32; }
+static bool ar_few(const AttnRowsParams& p) { return p.n * (p.n_head / p.n_kv) <= 32; }
+
+// Parts: a cut takes at most kArBlocks column blocks of 32 of either kind, or one split.
+static size_t ar_parts_bytes(const AttnRowsParams& p) {
+  const long long heads = (long long)p.batch * p.n * p.n_head;
+  const long long most = std::min((kArMaxPrefixSplits + kArMaxTailSplits) * heads, 2 * (heads + 32ll * kArBlocks));
+  return (size_t)most * (p.hd + 2) * 4;
+}
+static size_t ar_score_bytes(const AttnRowsParams& p) {
+  const int rep = p.n_head / p.n_kv;
+  return (size_t)std::min(p.n * rep, 32) * p.n_kv * ar_score_ld(p) * 4;
+}
+size_t attn_rows_work_bytes(const AttnRowsParams& p) { return ar_parts_bytes(p); }
+size_t attn_mass_work_bytes(const AttnRowsParams& p) { return ar_score_bytes(p) + (size_t)p.n * p.n_head * 8; }
+
+template <int HD, bool HALF, bool MASS>
+static int ar_launch(AttnRowsParams& p, hipStream_t s) {
+  p.prefix_cb = cdiv(p.cols, 32);
+  p.tail_cb = cdiv(p.n * p.rep, 32);
+  p.prefix_blocks = p.prefix_splits * p.prefix_cb * p.n_kv;
+  const int blocks = p.prefix_blocks + p.batch * p.tail_cb * p.n_kv * p.tail_splits;
+  hipLaunchKernelGGL((attn_rows_few_kernel<HD, HALF, MASS>), dim3(blocks), dim3(256), 0, s, p);
+  TRX_LAUNCHED();
+  const int join = p.nsplit > 1 ? (int)(((long long)p.batch * p.n * p.n_head + 3) / 4) : 0;
+  const int append = (int)(((long long)p.batch * p.n * p.n_kv * (HD / 8) + 255) / 256);
+  const int masses = p.scores ? cdiv(ar_most_rows(p), 256) * p.n_kv : 0;
+  hipLaunchKernelGGL((attn_rows_finish<HD, HALF, MASS>), dim3(join + append + masses), dim3(256), 0, s, p, join, append);
+  TRX_LAUNCHED();
+  if constexpr (MASS) {
+    if (!p.scores) {
+      hipLaunchKernelGGL((attn_mass_kernel<HD, HALF>), dim3(cdiv(ar_most_rows(p), 4 * kAwKeys) * p.n_kv), dim3(256), 0, s, p);
+      TRX_LAUNCHED();
+    }
+  }
+  return TRX_OK;
+}
+
+template <int HD, bool HALF>
+static int ar_launch(AttnRowsParams& p, hipStream_t s) {
+  return p.mass ? ar_launch<HD, HALF, true>(p, s) : ar_launch<HD, HALF, false>(p, s);
+}
+
+int launch_attn_rows(const AttnRowsParams& params, hipStream_t s) {
+  AttnRowsParams p = params;
+  const char* why = attn_rows_refuses(p);
+  TRX_CHECK(!why, TRX_E_INVALID, "attention over rows: %s", why);
+  if (p.n == 0 || p.batch == 0) return TRX_OK;
+  p.rep = p.n_head / p.n_kv;
+  p.cols = p.batch * p.n * p.rep;
+  p.rep_s = 32;
+  while (1 << (p.rep_s - 32) < p.rep) ++p.rep_s;
+  p.rep_m = ((1ull << p.rep_s) + p.rep - 1) / p.rep;
+  const ArPlan plan = ar_plan(p);
+  p.prefix_splits = plan.prefix;
+  p.tail_splits = plan.tail;
+  p.nsplit = plan.prefix + plan.tail;
+  if (p.mass) {
+    char* at = (char*)p.work + ar_parts_bytes(p);
+    p.scores = ar_few(p) ? (float*)at : nullptr;
+    p.score_ld = ar_score_ld(p);
+    p.norms = (float2*)(at + ar_score_bytes(p));
+  }
+  if (p.half_io) {
+    if (p.hd == 64) return ar_launch<64, true>(p, s);
+    if (p.hd == 128) return ar_launch<128, true>(p, s);
+    return ar_launch<256, true>(p, s);
+  }
+  if (p.hd == 64) return ar_launch<64, false>(p, s);
+  if (p.hd == 128) return ar_launch<128, false>(p, s);
+  return ar_launch<256, false>(p, s);
+}
+
+}  // namespace trx
+
+using namespace trx;
+
+#define TRX_API extern "C" __attribute__((visibility("default")))
+
+static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+template <class Shape>
+static AttnRowsParams rows_params(const Shape* a, int batch, int n) {
+  AttnRowsParams p = {};
+  p.half_io = a->kind == TRX_KIND_F16;
+  p.batch = batch;
+  p.n = n;
+  p.n_head = a->n_head;
+  p.n_kv = a->n_kv_head;
+  p.hd = a->head_dim;
+  p.q_stride = a->q_stride;
+  p.kv_stride = a->kv_stride;
+  p.out_stride = a->out_stride;
+  p.gate_stride = a->gate_stride;
+  p.gate_head_stride = a->gate_head_stride;
+  p.scale = a->scale;
+  return p;
+}
+static AttnRowsParams shared_params(const trx_attn_shared_shape* a, int batch, int n, int prefix) {
+  AttnRowsParams p = rows_params(a, batch, n);
+  p.prefix_slots = a->prefix_slots;
+  p.tail_slots = a->tail_slots;
+  p.prefix = prefix;
+  return p;
+}
+static AttnRowsParams mass_params(const trx_attn_mass_shape* a, int n) {
+  AttnRowsParams p = rows_params(a, 1, n);
+  p.tail_slots = a->slots;
+  return p;
+}
+
+#define TRX_CHECK_SHAPE(shape, name)                                                                              \
+  do {                                                                                                            \
+    TRX_CHECK(shape, TRX_E_INVALID, name ": null shape");                                                         \
+    TRX_CHECK((shape)->kind == TRX_KIND_F32 || (shape)->kind == TRX_KIND_F16, TRX_E_INVALID,                      \
+              name ": kind %d is not F32 or F16", (shape)->kind);                                                 \
+  } while (0)
+
+TRX_API int trx_attn_shared_geometry(const trx_attn_shared_shape* shape, int batch, int n, int prefix, size_t* workspace_bytes) {
+  TRX_CHECK_SHAPE(shape, "trx_attn_shared_geometry");
+  TRX_CHECK(workspace_bytes, TRX_E_INVALID, "trx_attn_shared_geometry: null argument");
+  const AttnRowsParams p = shared_params(shape, batch, n, prefix);
+  const char* why = attn_rows_refuses(p);
+  TRX_CHECK(!why, TRX_E_INVALID, "trx_attn_shared_geometry: %s", why);
+  *workspace_bytes = attn_rows_work_bytes(p);
+  return TRX_OK;
+}
+
+TRX_API int trx_attn_shared(const trx_attn_shared_shape* shape, int batch, int n, int prefix, const int32_t* lengths,
+                            const int32_t* counts, const void* q, const uint16_t* k, const uint16_t* v,
+                            const uint16_t* kprefix, const uint16_t* vprefix, uint16_t* ktail, uint16_t* vtail,
+                            const void* gate, void* out, void* workspace, trx_stream_t s) {
+  TRX_CHECK_SHAPE(shape, "trx_attn_shared");
+  AttnRowsParams p = shared_params(shape, batch, n, prefix);
+  p.gate = gate;
+  const char* why = attn_rows_refuses(p);
+  TRX_CHECK(!why, TRX_E_INVALID, "trx_attn_shared: %s", why);
+  if (batch == 0 || n == 0) return TRX_OK;
+  TRX_CHECK(lengths && q && k && v && ktail && vtail && out && workspace && (prefix == 0 || (kprefix && vprefix)),
+            TRX_E_INVALID, "trx_attn_shared: null argument");
+  TRX_CHECK(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(kprefix) && aligned16(vprefix) && aligned16(ktail) &&
+            aligned16(vtail) && aligned16(gate) && aligned16(out) && aligned16(workspace), TRX_E_INVALID,
+            "trx_attn_shared: a pointer is not 16-byte aligned");
+  TRX_CHECK(((uintptr_t)lengths & 3) == 0 && ((uintptr_t)counts & 3) == 0, TRX_E_INVALID,
+            "trx_attn_shared: lengths or counts are not 4-byte aligned");
+  p.lengths = lengths;
+  p.counts = counts;
+  p.q = q;
+  p.out = out;
+  p.k = (const __half*)k;
+  p.v = (const __half*)v;
+  p.kprefix = (const __half*)kprefix;
+  p.vprefix = (const __half*)vprefix;
+  p.ktail = (__half*)ktail;
+  p.vtail = (__half*)vtail;
+  p.work = workspace;
+  return launch_attn_rows(p, (hipStream_t)s);
+}
+
+TRX_API int trx_attn_mass_geometry(const trx_attn_mass_shape* shape, int n, size_t* workspace_bytes) {
+  TRX_CHECK_SHAPE(shape, "trx_attn_mass_geometry");
+  TRX_CHECK(workspace_bytes, TRX_E_INVALID, "trx_attn_mass_geometry: null argument");
+  AttnRowsParams p = mass_params(shape, n);
+  const char* why = attn_rows_refuses(p);
+  TRX_CHECK(!why, TRX_E_INVALID, "trx_attn_mass_geometry: %s", why);
+  *workspace_bytes = attn_rows_work_bytes(p) + attn_mass_work_bytes(p);
+  return TRX_OK;
+}
+
+TRX_API int trx_attn_mass(const trx_attn_mass_shape* shape, int n, int count, int pos, const int32_t* state, const void* q,
+                          const uint16_t* k, const uint16_t* v, uint16_t* kcache, uint16_t* vcache, float* mass,
+                          int32_t* positions, const void* gate, void* out, void* workspace, trx_stream_t s) {
+  TRX_CHECK_SHAPE(shape, "trx_attn_mass");
+  AttnRowsParams p = mass_params(shape, n);
+  p.gate = gate;
+  const char* why = attn_rows_refuses(p);
+  TRX_CHECK(!why, TRX_E_INVALID, "trx_attn_mass: %s", why);
+  TRX_CHECK(n <= shape->slots, TRX_E_INVALID, "trx_attn_mass: %d rows, %d slots", n, shape->slots);
+  TRX_CHECK(state || (count >= 0 && count <= shape->slots - n), TRX_E_INVALID, "trx_attn_mass: %d rows and %d new ones, %d slots",
+            count, n, shape->slots);
+  TRX_CHECK(state || (pos >= 0 && pos <= INT_MAX - n), TRX_E_INVALID, "trx_attn_mass: position %d", pos);
+  if (n == 0) return TRX_OK;
+  TRX_CHECK(q && k && v && kcache && vcache && mass && positions && out && workspace, TRX_E_INVALID,
+            "trx_attn_mass: null argument");
+  TRX_CHECK(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(kcache) && aligned16(vcache) && aligned16(gate) &&
+            aligned16(out) && aligned16(workspace), TRX_E_INVALID, "trx_attn_mass: a pointer is not 16-byte aligned");
+  TRX_CHECK(((uintptr_t)mass & 3) == 0 && ((uintptr_t)positions & 3) == 0 && ((uintptr_t)state & 3) == 0, TRX_E_INVALID,
+            "trx_attn_mass: mass, positions or state are not 4-byte aligned");
+  p.state = state;
+  p.length = count;
+  p.pos = pos;
+  p.q = q;
+  p.out = out;
+  p.k = (const __half*)k;
+  p.v = (const __half*)v;
+  p.ktail = (__half*)kcache;
+  p.vtail = (__half*)vcache;
+  p.mass = mass;
+  p.positions = positions;
+  p.work = workspace;
+  return launch_attn_rows(p, (hipStream_t)s);
+}
