@@ -41,7 +41,8 @@ struct AttnRowsParams {
   int prefix_cb, tail_cb;      // column blocks of the batch and of a draft
   float* scores;               // [n_kv][cols][score_ld], powers of two, of calls of few columns with masses
   long long score_ld;
-  float2* norms;               // [n_kv][cols]: a probability is 2^(score - norm.x) norm.y
+  float4* norms;               // [n_kv][cols]: a probability is 2^(z raw score - x) y
+  void* planes;                // the queries as operands, of calls of many columns with masses
 };
 
 // Why a geometry is not taken (null: it is).

@@ -19,12 +19,17 @@ namespace trx {
 
 // The rows that sequence seq has and gets; whether it takes part.
 __device__ __forceinline__ bool ar_sequence(const AttnRowsParams& p, int seq, int& have, int& fresh) {
-  have = p.state ? p.state[0] : p.lengths ? p.lengths[seq] : p.length;
-  fresh = p.counts ? p.counts[seq] : p.n;
+  // (Read first: a choice between addresses would put the arguments into memory of the lane's own.)
+  have = __builtin_amdgcn_readfirstlane(p.length);
+  fresh = __builtin_amdgcn_readfirstlane(p.n);
+  if (p.state) have = p.state[0];
+  else if (p.lengths) have = p.lengths[seq];
+  if (p.counts) fresh = p.counts[seq];
   return have >= 0 && fresh > 0 && fresh <= p.n && have <= p.tail_slots - fresh;
 }
 __device__ __forceinline__ bool ar_position(const AttnRowsParams& p, int& pos) {
-  pos = p.state ? p.state[1] : p.pos;
+  pos = __builtin_amdgcn_readfirstlane(p.pos);
+  if (p.state) pos = p.state[1];
   return pos >= 0 && pos <= INT_MAX - p.n;
 }
 
@@ -120,6 +125,8 @@ struct ArLine {
     const int cb = (int)(i - (unsigned)b.seq * p.tail_cb);
     int fresh, pos;
     if (!ar_sequence(p, b.seq, b.cached, fresh) || (MASS && !ar_position(p, pos))) return false;
+    b.cached = __builtin_amdgcn_readfirstlane(b.cached);   // (loaded, so not known to be uniform)
+    fresh = __builtin_amdgcn_readfirstlane(fresh);
     b.row0 = b.seq * p.n;
     b.c0 = b.row0 * p.rep + cb * columns;
     b.end = (b.row0 + fresh) * p.rep;
@@ -139,6 +146,19 @@ struct ArLine {
   __device__ __forceinline__ static bool all_see(const Params&, const Block&, const Column& c, int x0) {
     return x0 + kAwKeys <= c.w_first;
   }
+  // Queries as the mass kernel takes them: a wave's 32 columns, plane by plane, chunk by chunk, 16 bytes a lane.
+  template <class Query>
+  __device__ __forceinline__ static void queries(const Params& p, const Block& b, int first, int lane, const Query& q, float cs) {
+    if (!MASS || !p.planes || b.split || first >= p.cols) return;
+    constexpr int NC = HD / 16, ALL = NC + (sizeof(q.lo) > sizeof(half8_t) ? NC : 0);
+    half8_t* to = (half8_t*)p.planes + ((size_t)b.g * ((p.cols + 31) / 32) + first / 32) * ALL * 64 + lane;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      to[k * 64] = q.hi[k];
+      if constexpr (ALL > NC) to[(NC + k) * 64] = q.lo[k];
+    }
+    if (lane < 32 && first + lane < p.cols) p.norms[(size_t)b.g * p.cols + first + lane].z = cs;
+  }
   // A lane's scores of keys x, x + 8, x + 16 and x + 24, four each, in powers of two.
   __device__ __forceinline__ static void scored(const Params& p, const Block& b, int col, int x, const f32x16_t& s, float cs) {
     if (MASS && p.scores) {
@@ -149,7 +169,7 @@ struct ArLine {
     }
   }
   __device__ __forceinline__ static void total(const Params& p, const Block& b, int col, const float2& ml) {
-    if constexpr (MASS) p.norms[(size_t)b.g * p.cols + col] = ar_norm(ml.x, ml.y);
+    if constexpr (MASS) *(float2*)(p.norms + (size_t)b.g * p.cols + col) = ar_norm(ml.x, ml.y);
   }
 };
 
@@ -159,7 +179,7 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ * WK / 4) void attn_rows_kernel(At
 }
 
 template <int HD, bool HALF, bool MASS>
-__global__ __launch_bounds__(256, 1) void attn_rows_few_kernel(AttnRowsParams p) {
+__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_rows_few_kernel(AttnRowsParams p) {
   aw_few<ArLine<HD, MASS>, HD, HALF>(p);
 }
 
@@ -189,7 +209,7 @@ __device__ __forceinline__ void ar_mass_few(const AttnRowsParams& p, int block, 
     }
     if ((threadIdx.x & 7) == 0) norm[c] = ar_norm(M, l);
   } else if ((threadIdx.x & 7) == 0 && c < p.cols) {
-    norm[c] = p.norms[(size_t)g * p.cols + c];
+    norm[c] = *(const float2*)(p.norms + (size_t)g * p.cols + c);
   }
   __syncthreads();
   if (x >= N) return;
@@ -218,7 +238,7 @@ __global__ __launch_bounds__(256) void attn_rows_finish(AttnRowsParams p, int jo
     aw_join<HD, HALF>(p, row, head, lane, M, l);
     if (MASS && lane == 0) {
       const int g = aw_row(p, head);
-      p.norms[(size_t)g * p.cols + row * p.rep + head - g * p.rep] = ar_norm(M, l);
+      *(float2*)(p.norms + (size_t)g * p.cols + row * p.rep + head - g * p.rep) = ar_norm(M, l);
     }
     return;
   }
@@ -242,76 +262,153 @@ __global__ __launch_bounds__(256) void attn_rows_finish(AttnRowsParams p, int jo
   if constexpr (MASS) ar_mass_few(p, blockIdx.x - join_blocks - append_blocks, norm);
 }
 
-// Many columns: the masses of 32 keys a wave, which holds the keys' rows while the columns pass, 32 at a time.
+// Many columns: the scores once more, with the keys' rows in registers (KT tiles of 32 a wave) while the columns pass
+// through LDS, 32 for each of CG groups of KW waves a stage; a lane adds up its column's probabilities of its keys,
+// lanes and groups are added at the end. The queries come as the attention left them, in operands' order.
 template <int HD, bool HALF>
-__global__ __launch_bounds__(256) void attn_mass_kernel(AttnRowsParams p) {
-  using Wave = AwWave<ArLine<HD, true>, HD, HALF, false>;
-  const int kb = blockIdx.x / (unsigned)p.n_kv, w = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 5, j = lane & 31;
+struct ArMass {
+  static constexpr int KT = HD == 256 ? 1 : 2, KW = HD == 256 ? 4 : 2, CG = 8 / KW;
+  static constexpr int KEYS = 32 * KT * KW;                    // a block's
+  static constexpr int NC = HD / 16, ALL = HALF ? NC : 2 * NC;  // KB of a stage's operands a group
+  static constexpr int B = CG * ALL * 1024;                    // bytes of a stage
+};
+template <int HD, bool HALF>
+__global__ __launch_bounds__(512, 2) void attn_mass_kernel(AttnRowsParams p) {
+  using A = ArMass<HD, HALF>;
+  __shared__ __align__(1024) uint8_t smem[2 * A::B];
+  __shared__ float part[A::CG][A::KEYS];
+  const int kb = blockIdx.x / (unsigned)p.n_kv, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int h = lane >> 5, j = lane & 31, kw = w % A::KW, cg = w / A::KW;
   ArBlock b;
   int pos, fresh;
   b.g = (int)blockIdx.x - kb * p.n_kv;
   b.seq = b.row0 = 0;
   b.tail = true;
   if (!ar_sequence(p, 0, b.cached, fresh) || !ar_position(p, pos)) return;
+  b.cached = __builtin_amdgcn_readfirstlane(b.cached);
   b.N = b.cached + fresh;
-  const int x0 = (kb * 4 + w) * kAwKeys;
-  if (x0 >= b.N) return;
+  if (kb * A::KEYS >= b.N) return;
+  const int x0 = kb * A::KEYS + 32 * A::KT * kw;
   const ArRows<HD> rows(p, b);
-  long long own;
-  const long long at = rows.row(b, x0 + j, own);
-  const char* kr = rows.kc + at + (rows.kd & own) + 16 * h;
-  half8_t kf[Wave::NC];
+  half8_t kf[A::KT][A::NC];
 #pragma unroll
-  for (int k = 0; k < Wave::NC; ++k) kf[k] = *(const half8_t*)(kr + 32 * k);
-  f32x16_t sum = {};
-  // Columns before the first new row that sees key x0 have nothing for the tile.
-  for (int c0 = max(0, x0 - b.cached) * p.rep; c0 < p.cols; c0 += 32) {
-    const int col = min(c0 + j, p.cols - 1), row = aw_row(p, col), head = b.g * p.rep + col - row * p.rep;
-    const char* qr = (const char*)p.q + ((size_t)row * p.q_stride + (size_t)head * HD) * (HALF ? 2 : 4);
-    AwQuery<HD, HALF> q;
-    const float cs = q.take(p.scale, h, [&](int i) { return *(const u32x4_t*)(qr + 16 * i); });
-    const float2 norm = p.norms[(size_t)b.g * p.cols + col];
-    const f32x16_t s = Wave::scores([&](int k) { return kf[k]; }, [&](int k) { return q.hi[k]; },
-                                    [&](int k) { return q.lo[HALF ? 0 : k]; });
-    const int lim = c0 + j < p.cols ? b.cached + row + 1 : 0;
+  for (int t = 0; t < A::KT; ++t) {
+    long long own;
+    const long long at = rows.row(b, x0 + 32 * t + j, own);
+    const char* kr = rows.kc + at + (rows.kd & own) + 16 * h;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int x = x0 + 8 * (e >> 2) + 4 * h + (e & 3);
-      sum[e] = x < lim ? fmaf(__builtin_amdgcn_exp2f(fmaf(s[e], cs, -norm.x)), norm.y, sum[e]) : sum[e];
+    for (int k = 0; k < A::NC; ++k) kf[t][k] = *(const half8_t*)(kr + 32 * k);
+  }
+  // Columns before the first new row that sees the block's first key have nothing for it.
+  const int cbs = (p.cols + 31) / 32, cb0 = max(0, kb * A::KEYS - b.cached) * p.rep / 32;
+  const char* planes = (const char*)p.planes + (size_t)b.g * cbs * A::ALL * 1024;
+  const float4* norms = p.norms + (size_t)b.g * p.cols;
+  const uint32_t lds = lds_address(smem);
+  // A stage's operands, 1 KB a load of a wave; column blocks past the last are that one again, its keys unseen.
+  auto load = [&](int cb, int half) AW_INLINE {
+    for (int i = w; i < A::CG * A::ALL; i += 8) {
+      const int group = i / A::ALL;
+      const size_t at = (size_t)min(cb + group, cbs - 1) * A::ALL + (i - group * A::ALL);
+      load_lds16(lds + half * A::B + 1024 * i, uniform(planes + at * 1024), (uint32_t)lane * 16);
+    }
+  };
+  float sum[A::KT][16] = {};
+  load(cb0, 0);
+  float4 norm = norms[min((cb0 + cg) * 32 + j, p.cols - 1)];
+  for (int cb = cb0, half = 0; cb < cbs; cb += A::CG, half ^= 1) {
+    wait_loads_and_block<0>();
+    if (cb + A::CG < cbs) load(cb + A::CG, half ^ 1);
+    const int col = (cb + cg) * 32 + j;
+    const float4 now = norm;
+    norm = norms[min(col + 32 * A::CG, p.cols - 1)];
+    const uint32_t at = lds + half * A::B + cg * A::ALL * 1024 + lane * 16;
+    f32x16_t s[A::KT] = {};
+#pragma unroll
+    for (int k = 0; k < A::NC; ++k) {
+      const half8_t hi = lds_half8(at + 1024 * k);
+#pragma unroll
+      for (int t = 0; t < A::KT; ++t) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[t][k], hi, s[t], 0, 0, 0);
+      if constexpr (!HALF) {
+        const half8_t lo = lds_half8(at + 1024 * (A::NC + k));
+#pragma unroll
+        for (int t = 0; t < A::KT; ++t) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[t][k], lo, s[t], 0, 0, 0);
+      }
+    }
+    const int lim = col < p.cols ? b.cached + aw_row(p, col) + 1 : 0;
+    if (__all(lim >= x0 + 32 * A::KT)) {
+#pragma unroll
+      for (int t = 0; t < A::KT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          sum[t][e] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[t][e], now.z, -now.x)), now.y, sum[t][e]);
+    } else {
+#pragma unroll
+      for (int t = 0; t < A::KT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (x0 + 32 * t + 8 * (e >> 2) + 4 * h + (e & 3) < lim)
+            sum[t][e] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[t][e], now.z, -now.x)), now.y, sum[t][e]);
     }
   }
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1)
+  for (int t = 0; t < A::KT; ++t)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) sum[e] += __shfl_xor(sum[e], o, 64);
-  if (j) return;
-  float* m = p.mass + (size_t)b.g * p.tail_slots;
+    for (int e = 0; e < 16; ++e) {
+      float v = row16_sum(sum[t][e]);
+      v += __shfl_xor(v, 16, 64);
+      if (j == 0) part[cg][32 * (A::KT * kw + t) + 8 * (e >> 2) + 4 * h + (e & 3)] = v;
+    }
+  __syncthreads();
+  const int x = kb * A::KEYS + threadIdx.x;
+  if (threadIdx.x >= A::KEYS || x >= b.N) return;
+  float v = 0.f;
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const int x = x0 + 8 * (e >> 2) + 4 * h + (e & 3);
-    if (x < b.N) m[x] = x < b.cached ? m[x] + sum[e] : sum[e];
-  }
+  for (int i = 0; i < A::CG; ++i) v += part[i][threadIdx.x];
+  float* m = p.mass + (size_t)b.g * p.tail_slots + x;
+  *m = x < b.cached ? *m + v : v;
 }
 
 // Launch ------------------------------------------------------------------------------------------
 
-constexpr int kArBlocks = 512;                      // blocks that a cut of the keys aims at
-constexpr int kArMaxPrefixSplits = 64, kArMaxTailSplits = 16;
+constexpr int kArCus = 256;
+constexpr int kArMaxSplits = 64;
+constexpr int kArPartRows = 32768;                  // (column, split) pairs of all kv heads that a split segment takes
 
-// How a call is cut: splits of the prefix's and of the tails' keys, in column blocks of 32.
-struct ArPlan {
-  int prefix, tail;
+// How a segment (the prefix under all columns, or the tails under their own) is cut: columns a block, in waves of 32
+// (1: the kernel for few columns), and splits of the keys.
+struct ArCut {
+  int wq, splits;
 };
-static int ar_splits(long long blocks, int keys, int most) {
-  const int tiles = cdiv(keys, kAwKeys);
-  return (int)std::max(1ll, std::min({(long long)most, kArBlocks / std::max(blocks, 1ll), (long long)tiles / 4}));
-}
+
 // The rows that a tail has at most after the call.
 static int ar_most_rows(const AttnRowsParams& p) { return p.state || p.lengths ? p.tail_slots : p.length + p.n; }
-static ArPlan ar_plan(const AttnRowsParams& p) {
+
+static ArCut ar_cut(const AttnRowsParams& p, int units, int cols, int keys, bool few) {
+  ArCut best = {1, 1};
+  double least = 1e300;
+  for (int wq : {1, 2, 4}) {
+    if (few && wq > 1) break;
+    const int wk = wq == 1 ? 4 : (p.hd == 256 ? 4 : 8) / wq;
+    const double fixed = wq == 1 ? 2 : 11;
+    const double unit = wq == 1 ? p.hd / 64.0 : 1.35 * (p.half_io ? 0.56 : 1.0) * (p.hd == 64 ? 0.6 : 1.0);
+    const double step = wq == 2 ? unit * (p.half_io ? 1.75 : p.hd == 256 ? 1.7 : 1.3) : unit;
+    const int tiles = cdiv(keys, kAwKeys);
+    const long long blocks = (long long)units * cdiv(cols, 32 * wq) * p.n_kv, rows = (long long)units * cols * p.n_kv;
+    for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+      if (s > 1 && (s > tiles || s * rows > kArPartRows)) break;
+      const int steps = cdiv(cdiv(tiles, s), wk);
+      const double full = (double)blocks * s / (kArCus * (wq == 1 && p.hd < 256 ? 2 : 1));
+      const double rounds = full <= 1 ? 1 : 0.5 * (full + std::ceil(full));
+      const double t = rounds * (fixed + steps * step * (1 + 0.4 * std::min(full, 1.0))) + 8.0 * s * rows * p.hd / 3e6;
+      if (t < least) least = t, best = {wq, s};
+    }
+  }
+  return best;
+}
+static void ar_plan(const AttnRowsParams& p, ArCut& prefix, ArCut& tail) {
   const int rep = p.n_head / p.n_kv;
-  const long long prefix = (long long)cdiv(p.batch * p.n * rep, 32) * p.n_kv, tail = (long long)p.batch * cdiv(p.n * rep, 32) * p.n_kv;
-  return {p.prefix > 0 ? ar_splits(prefix, p.prefix, kArMaxPrefixSplits) : 0, ar_splits(tail, ar_most_rows(p), kArMaxTailSplits)};
+  prefix = p.prefix > 0 ? ar_cut(p, 1, p.batch * p.n * rep, p.prefix, false) : ArCut{1, 0};
+  tail = ar_cut(p, p.batch, p.n * rep, ar_most_rows(p), p.mass && p.n * rep <= 32);
 }
 
 const char* attn_rows_refuses(const AttnRowsParams& p) {
@@ -336,26 +433,43 @@ const char* attn_rows_refuses(const AttnRowsParams& p) {
 static long long ar_score_ld(const AttnRowsParams& p) { return ((long long)p.tail_slots + 31) / 32 * 32; }
 static bool ar_few(const AttnRowsParams& p) { return p.n * (p.n_head / p.n_kv) <= 32; }
 
-// Parts: a cut takes at most kArBlocks column blocks of 32 of either kind, or one split.
+// Parts of the prefix and of the tails: one split of each, or as many as kArPartRows allows.
 static size_t ar_parts_bytes(const AttnRowsParams& p) {
-  const long long heads = (long long)p.batch * p.n * p.n_head;
-  const long long most = std::min((kArMaxPrefixSplits + kArMaxTailSplits) * heads, 2 * (heads + 32ll * kArBlocks));
-  return (size_t)most * (p.hd + 2) * 4;
+  const long long rows = (long long)p.batch * p.n * p.n_head;
+  return (size_t)(2 * std::min(std::max<long long>(rows, kArPartRows), kArMaxSplits * rows)) * (p.hd + 2) * 4;
 }
 static size_t ar_score_bytes(const AttnRowsParams& p) {
   const int rep = p.n_head / p.n_kv;
   return (size_t)std::min(p.n * rep, 32) * p.n_kv * ar_score_ld(p) * 4;
 }
 size_t attn_rows_work_bytes(const AttnRowsParams& p) { return ar_parts_bytes(p); }
-size_t attn_mass_work_bytes(const AttnRowsParams& p) { return ar_score_bytes(p) + (size_t)p.n * p.n_head * 8; }
+static size_t ar_norm_bytes(const AttnRowsParams& p) { return (size_t)p.n * p.n_head * sizeof(float4); }
+static size_t ar_plane_bytes(const AttnRowsParams& p) {
+  return (size_t)cdiv(p.n * (p.n_head / p.n_kv), 32) * 32 * p.n_kv * p.hd * (p.half_io ? 2 : 4);
+}
+size_t attn_mass_work_bytes(const AttnRowsParams& p) { return ar_score_bytes(p) + ar_norm_bytes(p) + ar_plane_bytes(p); }
+
+// One segment's blocks, or those of both (few columns each).
+template <int HD, bool HALF, bool MASS>
+static void ar_segment(AttnRowsParams& p, int wq, bool prefix, bool tail, hipStream_t s) {
+  constexpr int WT = HD == 256 ? 4 : 8;             // waves of the kernel for many columns
+  p.prefix_cb = cdiv(p.cols, 32 * wq);
+  p.tail_cb = cdiv(p.n * p.rep, 32 * wq);
+  p.prefix_blocks = prefix ? p.prefix_splits * p.prefix_cb * p.n_kv : 0;
+  const dim3 grid(p.prefix_blocks + (tail ? p.batch * p.tail_cb * p.n_kv * p.tail_splits : 0));
+  if (wq == 1) hipLaunchKernelGGL((attn_rows_few_kernel<HD, HALF, MASS>), grid, dim3(256), 0, s, p);
+  else if (wq == 2) hipLaunchKernelGGL((attn_rows_kernel<HD, HALF, MASS, 2, WT / 2, HD == 64 ? 2 : 1>), grid, dim3(64 * WT), 0, s, p);
+  else hipLaunchKernelGGL((attn_rows_kernel<HD, HALF, MASS, 4, WT / 4, 2>), grid, dim3(64 * WT), 0, s, p);
+}
 
 template <int HD, bool HALF, bool MASS>
-static int ar_launch(AttnRowsParams& p, hipStream_t s) {
-  p.prefix_cb = cdiv(p.cols, 32);
-  p.tail_cb = cdiv(p.n * p.rep, 32);
-  p.prefix_blocks = p.prefix_splits * p.prefix_cb * p.n_kv;
-  const int blocks = p.prefix_blocks + p.batch * p.tail_cb * p.n_kv * p.tail_splits;
-  hipLaunchKernelGGL((attn_rows_few_kernel<HD, HALF, MASS>), dim3(blocks), dim3(256), 0, s, p);
+static int ar_launch(AttnRowsParams& p, const ArCut& prefix, const ArCut& tail, hipStream_t s) {
+  const bool both = prefix.splits == 0 || (prefix.wq == 1 && tail.wq == 1);
+  if (!both) {
+    ar_segment<HD, HALF, MASS>(p, prefix.wq, true, false, s);
+    TRX_LAUNCHED();
+  }
+  ar_segment<HD, HALF, MASS>(p, tail.wq, both && prefix.splits > 0, true, s);
   TRX_LAUNCHED();
   const int join = p.nsplit > 1 ? (int)(((long long)p.batch * p.n * p.n_head + 3) / 4) : 0;
   const int append = (int)(((long long)p.batch * p.n * p.n_kv * (HD / 8) + 255) / 256);
@@ -364,7 +478,7 @@ static int ar_launch(AttnRowsParams& p, hipStream_t s) {
   TRX_LAUNCHED();
   if constexpr (MASS) {
     if (!p.scores) {
-      hipLaunchKernelGGL((attn_mass_kernel<HD, HALF>), dim3(cdiv(ar_most_rows(p), 4 * kAwKeys) * p.n_kv), dim3(256), 0, s, p);
+      hipLaunchKernelGGL((attn_mass_kernel<HD, HALF>), dim3(cdiv(ar_most_rows(p), ArMass<HD, HALF>::KEYS) * p.n_kv), dim3(512), 0, s, p);
       TRX_LAUNCHED();
     }
   }
@@ -372,8 +486,8 @@ static int ar_launch(AttnRowsParams& p, hipStream_t s) {
 }
 
 template <int HD, bool HALF>
-static int ar_launch(AttnRowsParams& p, hipStream_t s) {
-  return p.mass ? ar_launch<HD, HALF, true>(p, s) : ar_launch<HD, HALF, false>(p, s);
+static int ar_launch(AttnRowsParams& p, const ArCut& prefix, const ArCut& tail, hipStream_t s) {
+  return p.mass ? ar_launch<HD, HALF, true>(p, prefix, tail, s) : ar_launch<HD, HALF, false>(p, prefix, tail, s);
 }
 
 int launch_attn_rows(const AttnRowsParams& params, hipStream_t s) {
@@ -386,24 +500,26 @@ int launch_attn_rows(const AttnRowsParams& params, hipStream_t s) {
   p.rep_s = 32;
   while (1 << (p.rep_s - 32) < p.rep) ++p.rep_s;
   p.rep_m = ((1ull << p.rep_s) + p.rep - 1) / p.rep;
-  const ArPlan plan = ar_plan(p);
-  p.prefix_splits = plan.prefix;
-  p.tail_splits = plan.tail;
-  p.nsplit = plan.prefix + plan.tail;
+  ArCut prefix, tail;
+  ar_plan(p, prefix, tail);
+  p.prefix_splits = prefix.splits;
+  p.tail_splits = tail.splits;
+  p.nsplit = prefix.splits + tail.splits;
   if (p.mass) {
     char* at = (char*)p.work + ar_parts_bytes(p);
     p.scores = ar_few(p) ? (float*)at : nullptr;
     p.score_ld = ar_score_ld(p);
-    p.norms = (float2*)(at + ar_score_bytes(p));
+    p.norms = (float4*)(at + ar_score_bytes(p));
+    p.planes = ar_few(p) ? nullptr : at + ar_score_bytes(p) + ar_norm_bytes(p);
   }
   if (p.half_io) {
-    if (p.hd == 64) return ar_launch<64, true>(p, s);
-    if (p.hd == 128) return ar_launch<128, true>(p, s);
-    return ar_launch<256, true>(p, s);
+    if (p.hd == 64) return ar_launch<64, true>(p, prefix, tail, s);
+    if (p.hd == 128) return ar_launch<128, true>(p, prefix, tail, s);
+    return ar_launch<256, true>(p, prefix, tail, s);
   }
-  if (p.hd == 64) return ar_launch<64, false>(p, s);
-  if (p.hd == 128) return ar_launch<128, false>(p, s);
-  return ar_launch<256, false>(p, s);
+  if (p.hd == 64) return ar_launch<64, false>(p, prefix, tail, s);
+  if (p.hd == 128) return ar_launch<128, false>(p, prefix, tail, s);
+  return ar_launch<256, false>(p, prefix, tail, s);
 }
 
 }  // namespace trx

@@ -9,8 +9,9 @@
 //     0 .. N - 1; split of splits, its share of them, and sp, the part that its sums are;
 //   Rows: the places of the keys' rows (row, flat); Column: row, head and the columns it stands with;
 //   block (false: nothing to do), sight (whether a column sees a key), whole (stages that every column of a wave
-//     sees whole), all_see (one tile), scored (a tile's scores, in calls of few columns), total (of a column that one
-//     block finishes: its maximum and sum).
+//     sees whole), all_see (one tile); and what a layout may keep of the work: queries (a wave's, as operands),
+//     scored (a tile's scores, in calls of few columns), total (of a column that one block finishes: its maximum and
+//     sum).
 #pragma once
 
 #include "trx_internal.h"
@@ -516,6 +517,7 @@ __device__ __forceinline__ void aw_many(const typename Layout::Params& p) {
     wait_loads_and_block<0>();
     const uint32_t mine = ks + (32 * wq + j) * QROW;
     v.init(q.take(p.scale, h, [&](int i) { return __builtin_bit_cast(u32x4_t, lds_half8(mine + 16 * (i ^ swizzle(j)))); }));
+    if (wk == 0) Layout::queries(p, b, b.c0 + 32 * wq, lane, q, v.cs);
     wait_loads_and_block<0>();
   }
 
@@ -733,6 +735,7 @@ __device__ __forceinline__ void aw_few(const typename Layout::Params& p) {
     AwQuery<HD, HALF> q;
     const uint32_t at = lds_address(smem) + mine * QROW;
     v.init(q.take(p.scale, h, [&](int i) { return __builtin_bit_cast(u32x4_t, lds_half8(at + 16 * (i ^ swizzle(mine)))); }));
+    if (wk == 0) Layout::queries(p, b, b.c0, lane, q, v.cs);
 #pragma unroll
     for (int k = 0; k < Wave::NC; ++k)
       if (k % WK == wk) {

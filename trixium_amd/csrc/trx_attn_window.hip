@@ -155,6 +155,8 @@ struct AwRing {
     const int u0 = x0 - b.ns + b.lo;
     return x0 >= b.ns && u0 > c.w_last - p.window && u0 <= c.w_first - (kAwKeys - 1);
   }
+  template <class Query>
+  __device__ __forceinline__ static void queries(const Params&, const Block&, int, int, const Query&, float) {}
   __device__ __forceinline__ static void scored(const Params&, const Block&, int, int, const f32x16_t&, float) {}
   __device__ __forceinline__ static void total(const Params&, const Block&, int, const float2&) {}
 };
