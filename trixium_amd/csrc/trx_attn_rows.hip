@@ -269,8 +269,9 @@ template <int HD, bool HALF>
 struct ArMass {
   static constexpr int KT = HD == 256 ? 1 : 2, KW = HD == 256 ? 4 : 2, CG = 8 / KW;
   static constexpr int KEYS = 32 * KT * KW;                    // a block's
-  static constexpr int NC = HD / 16, ALL = HALF ? NC : 2 * NC;  // KB of a stage's operands a group
-  static constexpr int B = CG * ALL * 1024;                    // bytes of a stage
+  static constexpr int NC = HD / 16, ALL = HALF ? NC : 2 * NC;  // KB of 32 columns' operands
+  static constexpr int SB = HALF ? 2 : 1;                      // steps of CG column blocks a stage
+  static constexpr int B = SB * CG * ALL * 1024;               // bytes of a stage
 };
 template <int HD, bool HALF>
 __global__ __launch_bounds__(512, 2) void attn_mass_kernel(AttnRowsParams p) {
@@ -304,52 +305,97 @@ __global__ __launch_bounds__(512, 2) void attn_mass_kernel(AttnRowsParams p) {
   const char* planes = (const char*)p.planes + (size_t)b.g * cbs * A::ALL * 1024;
   const float4* norms = p.norms + (size_t)b.g * p.cols;
   const uint32_t lds = lds_address(smem);
-  // A stage's operands, 1 KB a load of a wave; column blocks past the last are that one again, its keys unseen.
-  auto load = [&](int cb, int half) AW_INLINE {
-    for (int i = w; i < A::CG * A::ALL; i += 8) {
-      const int group = i / A::ALL;
-      const size_t at = (size_t)min(cb + group, cbs - 1) * A::ALL + (i - group * A::ALL);
-      load_lds16(lds + half * A::B + 1024 * i, uniform(planes + at * 1024), (uint32_t)lane * 16);
+  // The operands of the stage that step i begins, 1 KB a load of a wave; column blocks past the last are that one
+  // again, its keys unseen.
+  auto load = [&](int i) AW_INLINE {
+    if (cb0 + i * A::CG >= cbs) return;
+    const uint32_t to = lds + (i / A::SB & 1) * A::B;
+    for (int k = w; k < A::B / 1024; k += 8) {
+      const int group = k / A::ALL;
+      const size_t at = (size_t)min(cb0 + i * A::CG + group, cbs - 1) * A::ALL + (k - group * A::ALL);
+      load_lds16(to + 1024 * k, uniform(planes + at * 1024), (uint32_t)lane * 16);
     }
   };
   float sum[A::KT][16] = {};
-  load(cb0, 0);
-  float4 norm = norms[min((cb0 + cg) * 32 + j, p.cols - 1)];
-  for (int cb = cb0, half = 0; cb < cbs; cb += A::CG, half ^= 1) {
-    wait_loads_and_block<0>();
-    if (cb + A::CG < cbs) load(cb + A::CG, half ^ 1);
-    const int col = (cb + cg) * 32 + j;
-    const float4 now = norm;
-    norm = norms[min(col + 32 * A::CG, p.cols - 1)];
-    const uint32_t at = lds + half * A::B + cg * A::ALL * 1024 + lane * 16;
-    f32x16_t s[A::KT] = {};
+  // The scores of a wave's next 32 columns are taken while the exponentials of these run, some after each chunk's
+  // products.
+  f32x16_t s[A::KT];
+  auto add = [&](const f32x16_t* of, int t, int e, const float4& norm) AW_INLINE {
+    sum[t][e] = fmaf(__builtin_amdgcn_exp2f(fmaf(of[t][e], norm.z, -norm.x)), norm.y, sum[t][e]);
+    asm volatile("" : "+v"(sum[t][e]));           // here, not where the sums are used next
+  };
+  auto scores = [&](int i, f32x16_t* to, auto beside) AW_INLINE {
+    const uint32_t at = lds + i % (2 * A::SB) * (A::B / A::SB) + cg * A::ALL * 1024 + lane * 16;
+    // Operands two steps ahead of their products; the barriers keep the steps as they stand here.
+    auto operand = [&](int k) AW_INLINE { return lds_half8(at + 1024 * (HALF ? k : k % 2 * A::NC + k / 2)); };
+    half8_t q[3] = {operand(0), operand(1), {}};
 #pragma unroll
-    for (int k = 0; k < A::NC; ++k) {
-      const half8_t hi = lds_half8(at + 1024 * k);
+    for (int k = 0; k < A::ALL; ++k) {
+      if (k + 2 < A::ALL) q[(k + 2) % 3] = operand(k + 2);
 #pragma unroll
-      for (int t = 0; t < A::KT; ++t) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[t][k], hi, s[t], 0, 0, 0);
-      if constexpr (!HALF) {
-        const half8_t lo = lds_half8(at + 1024 * (A::NC + k));
-#pragma unroll
-        for (int t = 0; t < A::KT; ++t) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[t][k], lo, s[t], 0, 0, 0);
-      }
+      for (int t = 0; t < A::KT; ++t)
+        to[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[t][HALF ? k : k / 2], q[k % 3], k ? to[t] : f32x16_t{}, 0, 0, 0);
+      beside(k);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    const int lim = col < p.cols ? b.cached + aw_row(p, col) + 1 : 0;
-    if (__all(lim >= x0 + 32 * A::KT)) {
+  };
+  auto column = [&](int i) AW_INLINE { return (cb0 + i * A::CG + cg) * 32 + j; };
+  auto norm_of = [&](int i) AW_INLINE { return norms[min(column(i), p.cols - 1)]; };
+  const int steps = (cbs - cb0 + A::CG - 1) / A::CG;
+  load(0);
+  float4 norm = norm_of(0), after = norm_of(1), now;
+  wait_loads_and_block<0>();
+  load(A::SB);
+  scores(0, s, [](int) {});
+  int i = 0;
+  // Before a step's exponentials: where the next one begins a stage, its operands are there for every wave, and the
+  // stage behind takes the place of what was read last.
+  auto begin = [&]() AW_INLINE {
+    now = norm;
+    if ((i + 1) % A::SB == 0) {
+      wait_loads_and_block<0>();
+      load(i + 1 + A::SB);
+    }
+    norm = after;
+    after = norm_of(i + 2);
+  };
+  // Steps up to number `to` with a mask: where new rows do not see the wave's keys, and the last one.
+  auto masked = [&](int to) AW_INLINE {
+    for (; i < to; ++i) {
+      const int col = column(i), lim = col < p.cols ? b.cached + aw_row(p, col) + 1 : 0;
+      begin();
 #pragma unroll
       for (int t = 0; t < A::KT; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          sum[t][e] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[t][e], now.z, -now.x)), now.y, sum[t][e]);
-    } else {
-#pragma unroll
-      for (int t = 0; t < A::KT; ++t)
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (x0 + 32 * t + 8 * (e >> 2) + 4 * h + (e & 3) < lim)
-            sum[t][e] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[t][e], now.z, -now.x)), now.y, sum[t][e]);
+          if (x0 + 32 * t + 8 * (e >> 2) + 4 * h + (e & 3) < lim) add(s, t, e, now);
+      if (i + 1 < steps) scores(i + 1, s, [](int) {});
     }
+  };
+  auto whole = [&](f32x16_t* of, f32x16_t* next) AW_INLINE {
+    begin();
+    scores(i + 1, next, [&](int k) AW_INLINE {
+#pragma unroll
+      for (int x = k * 16 * A::KT / A::ALL; x < (k + 1) * 16 * A::KT / A::ALL; ++x) add(of, x / 16, x % 16, now);
+    });
+    ++i;
+  };
+  // Steps [i0, i1) are whole: every column sees every key of the wave, and another step follows.
+  const int from = (max(0, x0 + 32 * A::KT - 1 - b.cached) * p.rep + 31) / 32;
+  const int i0 = min(steps, max(0, from - cg - cb0 + A::CG - 1) / A::CG);
+  const int i1 = max(i0, min(steps - 1, max(0, p.cols / 32 - cg - cb0 + A::CG - 1) / A::CG));
+  masked(i0);
+  f32x16_t next[A::KT];
+  while (i + 1 < i1) {
+    whole(s, next);
+    whole(next, s);
   }
+  if (i < i1) {
+    whole(s, next);
+#pragma unroll
+    for (int t = 0; t < A::KT; ++t) s[t] = next[t];
+  }
+  masked(steps);
 #pragma unroll
   for (int t = 0; t < A::KT; ++t)
 #pragma unroll
