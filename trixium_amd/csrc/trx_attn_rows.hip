@@ -13,6 +13,7 @@
 #include "trx_attn_tile.h"
 
 #include <algorithm>
+#include <type_traits>
 #include <limits.h>
 
 namespace trx {
@@ -146,6 +147,10 @@ struct ArLine {
   __device__ __forceinline__ static bool all_see(const Params&, const Block&, const Column& c, int x0) {
     return x0 + kAwKeys <= c.w_first;
   }
+  // A column's parts beside each other, as the join reads them.
+  __device__ __forceinline__ static size_t sum_at(const Params& p, const Block& b, int col, size_t) {
+    return ((size_t)b.g * p.cols + col) * p.nsplit + b.sp;
+  }
   // Queries as the mass kernel takes them: a wave's 32 columns, plane by plane, chunk by chunk, 16 bytes a lane.
   template <class Query>
   __device__ __forceinline__ static void queries(const Params& p, const Block& b, int first, int lane, const Query& q, float cs) {
@@ -183,83 +188,157 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_rows_few_kernel(A
   aw_few<ArLine<HD, MASS>, HD, HALF>(p);
 }
 
-// Few columns: one more key's mass a thread, from the scores that the attention kept. The columns' parts are joined
-// anew by every block: 32 columns, 8 lanes each.
+// The parts of a (row, head) joined by one wave: a lane has the reference and the sum of parts lane and lane + 64, so
+// that all of a column's loads are on their way at once. A column of a draft that takes no part is not written.
+template <int HD, bool HALF, bool MASS>
+__device__ __forceinline__ void ar_join(const AttnRowsParams& p, int row, int head, int lane) {
+  constexpr int E = HD / 64, MANY = 16;               // dims a lane; parts a time
+  typedef typename std::conditional<HALF, _Float16, float>::type io_t;
+  const int g = aw_row(p, head), col = row * p.rep + head - g * p.rep, seq = row / p.n;
+  int have, fresh;
+  const bool takes = ar_sequence(p, seq, have, fresh) && row - seq * p.n < fresh;
+  const size_t all = (size_t)p.nsplit * p.n_kv * p.cols, step = (size_t)p.n_kv * p.cols, at = (size_t)g * p.cols + col;
+  const float2* ml = (const float2*)((const float*)p.work + all * HD) + at * p.nsplit;
+  const float* po = (const float*)p.work + at * HD + E * lane;
+  float2 a[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    a[k] = make_float2(-INFINITY, 0.f);
+    if (lane + 64 * k < p.nsplit) a[k] = ml[lane + 64 * k];
+  }
+  io_t gate[E], out[E];
+  if (p.gate) __builtin_memcpy(gate, (const io_t*)p.gate + (size_t)row * p.gate_stride + (size_t)head * p.gate_head_stride + E * lane, sizeof gate);
+  float x[MANY][E], f[2], o[E] = {};
+  auto load = [&](int s0) AW_INLINE {
+#pragma unroll
+    for (int k = 0; k < MANY; ++k)
+      if (s0 + k < p.nsplit) __builtin_memcpy(x[k], po + (size_t)(s0 + k) * step * HD, sizeof x[k]);
+  };
+  load(0);
+  const float M = wave_max(fmaxf(a[0].x, a[1].x));
+#pragma unroll
+  for (int k = 0; k < 2; ++k) f[k] = aw_rescale(a[k].x, M);
+  const float l = wave_sum(a[0].y * f[0] + a[1].y * f[1]);
+  for (int s0 = 0;;) {
+#pragma unroll
+    for (int k = 0; k < MANY; ++k)
+      if (s0 + k < p.nsplit) {
+        const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(s0 < 64 ? f[0] : f[1]), (s0 + k) & 63));
+#pragma unroll
+        for (int i = 0; i < E; ++i) o[i] += x[k][i] * w;
+      }
+    s0 += MANY;
+    if (s0 >= p.nsplit) break;
+    load(s0);
+  }
+  if (!takes) return;
+  const float inv = 1.0f / l;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const float v = o[i] * inv;
+    out[i] = (io_t)(p.gate ? v * sigmoidf_((float)gate[i]) : v);
+  }
+  __builtin_memcpy((io_t*)p.out + (size_t)row * p.out_stride + (size_t)head * HD + E * lane, out, sizeof out);
+  if (MASS && lane == 0) *(float2*)(p.norms + at) = ar_norm(M, l);
+}
+
+// Few columns: the masses of four keys a thread, from the scores that the attention kept. The columns' parts are joined
+// anew by every block: `per` lanes a column.
+constexpr int kArMassKeys = 1024;
 __device__ __forceinline__ void ar_mass_few(const AttnRowsParams& p, int block, float2* norm) {
+  const int kb = block / p.n_kv, g = block - kb * p.n_kv, x0 = kb * kArMassKeys + threadIdx.x;
+  const int per = p.cols <= 4 ? 64 : p.cols <= 8 ? 32 : p.cols <= 16 ? 16 : 8, c = (int)threadIdx.x / per, first = threadIdx.x % per;
+  // What does not wait for the norms: the first columns' scores and the masses there are (of slots, rows or not).
+  constexpr int PRE = 4;
+  const float* s = p.scores + (size_t)g * p.cols * p.score_ld;
+  float* const m = p.mass + (size_t)g * p.tail_slots;
+  float pre[PRE][4], old[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int x = min(x0 + 256 * k, p.tail_slots - 1);
+    old[k] = m[x];
+#pragma unroll
+    for (int i = 0; i < PRE; ++i) pre[i][k] = s[min(i, p.cols - 1) * p.score_ld + x];
+  }
   int have, fresh;
   if (!ar_sequence(p, 0, have, fresh)) return;
-  const int kb = block / p.n_kv, g = block - kb * p.n_kv, x = kb * 256 + threadIdx.x, N = have + fresh;
-  if (kb * 256 >= N) return;
-  const int c = threadIdx.x >> 3;
-  float M = -INFINITY, l = 0.f;
+  const int N = have + fresh;
+  if (kb * kArMassKeys >= N) return;
   if (p.nsplit > 1) {
     const size_t all = (size_t)p.nsplit * p.n_kv * p.cols;
-    const float2* ml = (const float2*)((const float*)p.work + all * p.hd) + (size_t)g * p.cols + c;
-    for (int s = threadIdx.x & 7; s < p.nsplit && c < p.cols; s += 8) {
-      const float2 a = ml[(size_t)s * p.n_kv * p.cols];
-      const float to = fmaxf(M, a.x);
-      l = l * aw_rescale(M, to) + a.y * aw_rescale(a.x, to);
-      M = to;
-    }
+    const float2* ml = (const float2*)((const float*)p.work + all * p.hd) + ((size_t)g * p.cols + min(c, p.cols - 1)) * p.nsplit;
+    float M = -INFINITY, l = 0.f;
+    for (int s0 = first; s0 < p.nsplit; s0 += 8 * per) {
+      float2 a[8];
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
+      for (int k = 0; k < 8; ++k) a[k] = s0 + k * per < p.nsplit ? ml[s0 + k * per] : make_float2(-INFINITY, 0.f);
+      float to = M;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) to = fmaxf(to, a[k].x);
+      l *= aw_rescale(M, to);
+      M = to;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) l += a[k].y * aw_rescale(a[k].x, M);
+    }
+    for (int o = 1; o < per; o <<= 1) {
       const float m1 = __shfl_xor(M, o, 64), l1 = __shfl_xor(l, o, 64), to = fmaxf(M, m1);
       l = l * aw_rescale(M, to) + l1 * aw_rescale(m1, to);
       M = to;
     }
-    if ((threadIdx.x & 7) == 0) norm[c] = ar_norm(M, l);
-  } else if ((threadIdx.x & 7) == 0 && c < p.cols) {
+    if (first == 0 && c < p.cols) norm[c] = ar_norm(M, l);
+  } else if (first == 0 && c < p.cols) {
     norm[c] = *(const float2*)(p.norms + (size_t)g * p.cols + c);
   }
   __syncthreads();
-  if (x >= N) return;
-  const float* s = p.scores + (size_t)g * p.cols * p.score_ld + x;
-  float sum = 0.f;
-  for (int i = 0; i < p.cols; ++i) sum = fmaf(__builtin_amdgcn_exp2f(s[i * p.score_ld] - norm[i].x), norm[i].y, sum);
-  float* m = p.mass + (size_t)g * p.tail_slots + x;
-  *m = x < have ? *m + sum : sum;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int x = x0 + 256 * k;
+    if (x >= N) return;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < PRE; ++i)
+      if (i < p.cols) sum = fmaf(__builtin_amdgcn_exp2f(pre[i][k] - norm[i].x), norm[i].y, sum);
+#pragma unroll 4
+    for (int i = PRE; i < p.cols; ++i) sum = fmaf(__builtin_amdgcn_exp2f(s[i * p.score_ld + x] - norm[i].x), norm[i].y, sum);
+    m[x] = x < have ? old[k] + sum : sum;
+  }
 }
 
 // After the attention: the parts of each (row, head) joined (a wave each, blocks of four), the new rows into the
 // tails' slots, and the masses of calls of few columns.
 template <int HD, bool HALF, bool MASS>
-__global__ __launch_bounds__(256) void attn_rows_finish(AttnRowsParams p, int join_blocks, int append_blocks) {
+__global__ __launch_bounds__(256) void attn_rows_finish(AttnRowsParams p, int mass_blocks, int join_blocks) {
   __shared__ float2 norm[32];
   int pos = 0;
   if (MASS && !ar_position(p, pos)) return;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  if ((int)blockIdx.x < join_blocks) {
-    const unsigned id = blockIdx.x * 4 + w;         // below 2^23 + 4
+  // (First, so that a kv head's masses are added up on the XCD that has its scores.)
+  if (MASS && (int)blockIdx.x < mass_blocks) {
+    ar_mass_few(p, blockIdx.x, norm);
+    return;
+  }
+  const int block = (int)blockIdx.x - mass_blocks;
+  if (block < join_blocks) {
+    const unsigned id = block * 4 + w;              // below 2^23 + 4
     if (id >= (unsigned)(p.batch * p.n * p.n_head)) return;
-    const int row = (int)(id / (unsigned)p.n_head), head = (int)id - row * p.n_head, seq = row / p.n;
-    int have, fresh;
-    if (!ar_sequence(p, seq, have, fresh) || row - seq * p.n >= fresh) return;
-    float M, l;
-    aw_join<HD, HALF>(p, row, head, lane, M, l);
-    if (MASS && lane == 0) {
-      const int g = aw_row(p, head);
-      *(float2*)(p.norms + (size_t)g * p.cols + row * p.rep + head - g * p.rep) = ar_norm(M, l);
-    }
+    const int row = (int)(id / (unsigned)p.n_head);
+    ar_join<HD, HALF, MASS>(p, row, (int)id - row * p.n_head, lane);
     return;
   }
-  if ((int)blockIdx.x < join_blocks + append_blocks) {
-    // 16 bytes of K and V a thread.
-    constexpr int SEG = HD / 8;
-    const long long id = (long long)(blockIdx.x - join_blocks) * 256 + threadIdx.x;
-    if (id >= (long long)p.batch * p.n * p.n_kv * SEG) return;
-    const unsigned at = (unsigned)(id / SEG);        // below 2^23
-    const int sd = (int)(id % SEG) * 8, row = (int)(at / (unsigned)p.n_kv), g = (int)at - row * p.n_kv, seq = row / p.n;
-    const int i = row - seq * p.n;
-    int have, fresh;
-    if (!ar_sequence(p, seq, have, fresh) || i >= fresh) return;
-    const size_t slot = ((size_t)seq * p.n_kv + g) * p.tail_slots + have + i;
-    const size_t from = (size_t)row * p.kv_stride + (size_t)g * HD + sd;
-    *(uint4*)(p.ktail + slot * HD + sd) = *(const uint4*)(p.k + from);
-    *(uint4*)(p.vtail + slot * HD + sd) = *(const uint4*)(p.v + from);
-    if (MASS && sd == 0) p.positions[slot] = pos + i;
-    return;
-  }
-  if constexpr (MASS) ar_mass_few(p, blockIdx.x - join_blocks - append_blocks, norm);
+  // 16 bytes of K and V a thread.
+  constexpr int SEG = HD / 8;
+  const long long id = (long long)(block - join_blocks) * 256 + threadIdx.x;
+  if (id >= (long long)p.batch * p.n * p.n_kv * SEG) return;
+  const unsigned at = (unsigned)(id / SEG);          // below 2^23
+  const int sd = (int)(id % SEG) * 8, row = (int)(at / (unsigned)p.n_kv), g = (int)at - row * p.n_kv, seq = row / p.n;
+  const int i = row - seq * p.n;
+  int have, fresh;
+  if (!ar_sequence(p, seq, have, fresh) || i >= fresh) return;
+  const size_t slot = ((size_t)seq * p.n_kv + g) * p.tail_slots + have + i;
+  const size_t from = (size_t)row * p.kv_stride + (size_t)g * HD + sd;
+  *(uint4*)(p.ktail + slot * HD + sd) = *(const uint4*)(p.k + from);
+  *(uint4*)(p.vtail + slot * HD + sd) = *(const uint4*)(p.v + from);
+  if (MASS && sd == 0) p.positions[slot] = pos + i;
 }
 
 // Many columns: the scores once more, with the keys' rows in registers (KT tiles of 32 a wave) while the columns pass
@@ -429,32 +508,63 @@ struct ArCut {
 // The rows that a tail has at most after the call.
 static int ar_most_rows(const AttnRowsParams& p) { return p.state || p.lengths ? p.tail_slots : p.length + p.n; }
 
-static ArCut ar_cut(const AttnRowsParams& p, int units, int cols, int keys, bool few) {
-  ArCut best = {1, 1};
-  double least = 1e300;
-  for (int wq : {1, 2, 4}) {
-    if (few && wq > 1) break;
-    const int wk = wq == 1 ? 4 : (p.hd == 256 ? 4 : 8) / wq;
-    const double fixed = wq == 1 ? 2 : 11;
-    const double unit = wq == 1 ? p.hd / 64.0 : 1.35 * (p.half_io ? 0.56 : 1.0) * (p.hd == 64 ? 0.6 : 1.0);
-    const double step = wq == 2 ? unit * (p.half_io ? 1.75 : p.hd == 256 ? 1.7 : 1.3) : unit;
-    const int tiles = cdiv(keys, kAwKeys);
-    const long long blocks = (long long)units * cdiv(cols, 32 * wq) * p.n_kv, rows = (long long)units * cols * p.n_kv;
-    for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
-      if (s > 1 && (s > tiles || s * rows > kArPartRows)) break;
-      const int steps = cdiv(cdiv(tiles, s), wk);
-      const double full = (double)blocks * s / (kArCus * (wq == 1 && p.hd < 256 ? 2 : 1));
-      const double rounds = full <= 1 ? 1 : 0.5 * (full + std::ceil(full));
-      const double t = rounds * (fixed + steps * step * (1 + 0.4 * std::min(full, 1.0))) + 8.0 * s * rows * p.hd / 3e6;
-      if (t < least) least = t, best = {wq, s};
-    }
-  }
-  return best;
+// What a cut of a segment takes by this estimate, in microseconds, with `others` blocks beside it: a block takes a fixed
+// part (its queries, the first rows' latency, the join of its waves, the outputs) and a step for each wk tiles of keys;
+// a full chip makes a step 1.4 times as long.
+static double ar_time(const AttnRowsParams& p, const ArCut& c, int units, int cols, int keys, long long others) {
+  const int wk = c.wq == 1 ? 4 : (p.hd == 256 ? 4 : 8) / c.wq;
+  const double fixed = c.wq == 1 ? 2 : 11;
+  const double unit = c.wq == 1 ? p.hd / 64.0 : 1.35 * (p.half_io ? 0.56 : 1.0) * (p.hd == 64 ? 0.6 : 1.0);
+  const double step = c.wq == 2 ? unit * (p.half_io ? 1.75 : p.hd == 256 ? 1.7 : 1.3) : unit;
+  const long long blocks = (long long)units * cdiv(cols, 32 * c.wq) * p.n_kv * c.splits + others;
+  const int steps = cdiv(cdiv(cdiv(keys, kAwKeys), c.splits), wk);
+  const double full = (double)blocks / kArCus, rounds = full <= 1 ? 1 : 0.5 * (full + std::ceil(full));
+  return rounds * (fixed + steps * step * (1 + 0.4 * std::min(full, 1.0)));
 }
+
+// f of every cut of a segment into splits that its parts have room for.
+template <class F>
+static void ar_cuts(int wq, int keys, long long rows, F f) {
+  for (int s : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64}) {
+    if (s > 1 && (s > cdiv(keys, kAwKeys) || s * rows > kArPartRows)) return;
+    f(ArCut{wq, s});
+  }
+}
+
 static void ar_plan(const AttnRowsParams& p, ArCut& prefix, ArCut& tail) {
-  const int rep = p.n_head / p.n_kv;
-  prefix = p.prefix > 0 ? ar_cut(p, 1, p.batch * p.n * rep, p.prefix, false) : ArCut{1, 0};
-  tail = ar_cut(p, p.batch, p.n * rep, ar_most_rows(p), p.mass && p.n * rep <= 32);
+  const int rep = p.n_head / p.n_kv, cols = p.n * rep, all = p.batch * cols, keys = ar_most_rows(p);
+  const long long rows = (long long)p.batch * p.n * p.n_head;
+  const double part = 8.0 * rows * p.hd / 6e6;       // a part of every column written and read, at 6 TB/s
+  // Each segment alone, one launch behind the other (a prefix brings the join with it).
+  double time = 0, least = 1e300;
+  for (int wq : {1, 2, 4}) {
+    if (wq > 1 && cols <= 32) break;
+    ar_cuts(wq, keys, rows, [&](const ArCut& c) {
+      const double t = ar_time(p, c, p.batch, cols, keys, 0) + (c.splits > 1 ? (p.prefix ? 0 : 2) + c.splits * part : 0);
+      if (t < least) least = t, tail = c;
+    });
+  }
+  prefix = {1, 0};
+  if (p.prefix > 0) {
+    time = least + 2;
+    least = 1e300;
+    for (int wq : {1, 2, 4})
+      ar_cuts(wq, p.prefix, rows, [&](const ArCut& c) {
+        const double t = ar_time(p, c, 1, all, p.prefix, 0) + c.splits * part;
+        if (t < least) least = t, prefix = c;
+      });
+    time += least;
+    // Both in one launch, of few columns a block.
+    ar_cuts(1, keys, rows, [&](const ArCut& b) {
+      const long long tails = (long long)p.batch * cdiv(cols, 32) * p.n_kv * b.splits;
+      ar_cuts(1, p.prefix, rows, [&](const ArCut& a) {
+        const long long prefixes = (long long)cdiv(all, 32) * p.n_kv * a.splits;
+        const double t = std::max(ar_time(p, a, 1, all, p.prefix, tails), ar_time(p, b, p.batch, cols, keys, prefixes)) +
+                         (a.splits + b.splits) * part;
+        if (t < time) time = t, prefix = a, tail = b;
+      });
+    });
+  }
 }
 
 const char* attn_rows_refuses(const AttnRowsParams& p) {
@@ -519,8 +629,8 @@ static int ar_launch(AttnRowsParams& p, const ArCut& prefix, const ArCut& tail, 
   TRX_LAUNCHED();
   const int join = p.nsplit > 1 ? (int)(((long long)p.batch * p.n * p.n_head + 3) / 4) : 0;
   const int append = (int)(((long long)p.batch * p.n * p.n_kv * (HD / 8) + 255) / 256);
-  const int masses = p.scores ? cdiv(ar_most_rows(p), 256) * p.n_kv : 0;
-  hipLaunchKernelGGL((attn_rows_finish<HD, HALF, MASS>), dim3(join + append + masses), dim3(256), 0, s, p, join, append);
+  const int masses = p.scores ? cdiv(ar_most_rows(p), kArMassKeys) * p.n_kv : 0;
+  hipLaunchKernelGGL((attn_rows_finish<HD, HALF, MASS>), dim3(masses + join + append), dim3(256), 0, s, p, masses, join);
   TRX_LAUNCHED();
   if constexpr (MASS) {
     if (!p.scores) {

@@ -16,8 +16,6 @@
 
 #include "trx_internal.h"
 
-#include <type_traits>
-
 namespace trx {
 
 constexpr int kAwKeys = 32;                 // keys per wave and stage
@@ -429,7 +427,7 @@ struct AwWave {
     if (p.nsplit > 1) {
       const size_t all = (size_t)p.nsplit * p.n_kv * p.cols, at = ((size_t)b.sp * p.n_kv + b.g) * p.cols + col;
       *(float4*)((float*)p.work + at * HD + d0) = x;
-      if (d0 == 0) *((float2*)((float*)p.work + all * HD) + at) = ml;
+      if (d0 == 0) *((float2*)((float*)p.work + all * HD) + Layout::sum_at(p, b, col, at)) = ml;
       return;
     }
     if (d0 == 0) Layout::total(p, b, col, ml);
@@ -818,62 +816,4 @@ __device__ __forceinline__ void aw_few(const typename Layout::Params& p) {
                 make_float4(x[4 * a4], x[4 * a4 + 1], x[4 * a4 + 2], x[4 * a4 + 3]), make_float2(M, l));
   }
 }
-// The parts of a (position, head) joined by one wave; M and l: its reference and the sum behind it.
-template <int HD, bool HALF, class Params>
-__device__ __forceinline__ void aw_join(const Params& p, int row, int head, int lane, float& M, float& l) {
-  constexpr int E = HD / 64;                       // dims a lane: E lane .. + E - 1
-  const int g = aw_row(p, head), col = row * p.rep + head - g * p.rep;
-  const size_t all = (size_t)p.nsplit * p.n_kv * p.cols, step = (size_t)p.n_kv * p.cols;
-  const size_t at = (size_t)g * p.cols + col;
-  const float2* ml = (const float2*)((const float*)p.work + all * HD) + at;
-  const float* po = (const float*)p.work + at * HD + E * lane;
-  const size_t gi = (size_t)row * p.gate_stride + (size_t)head * p.gate_head_stride + E * lane;
-  const size_t oi = (size_t)row * p.out_stride + (size_t)head * HD + E * lane;
-  typedef typename std::conditional<HALF, _Float16, float>::type io_t;
-  io_t gate[E], out[E];
-  if (p.gate) __builtin_memcpy(gate, (const io_t*)p.gate + gi, sizeof gate);
-  float o[E];
-  M = -INFINITY;
-  l = 0.f;
-#pragma unroll
-  for (int i = 0; i < E; ++i) o[i] = 0.f;
-  // Eight splits' loads at a time in flight (the gate's with them), a running reference over the eights.
-  for (int s0 = 0; s0 < p.nsplit; s0 += 8) {
-    float2 a[8];
-    float x[8][E];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      a[k] = make_float2(-INFINITY, 0.f);
-#pragma unroll
-      for (int i = 0; i < E; ++i) x[k][i] = 0.f;
-      if (s0 + k < p.nsplit) {
-        a[k] = ml[(s0 + k) * step];
-        __builtin_memcpy(x[k], po + (s0 + k) * step * HD, 4 * E);
-      }
-    }
-    float top = M;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) top = fmaxf(top, a[k].x);
-    const float keep = aw_rescale(M, top);
-    M = top;
-    l *= keep;
-#pragma unroll
-    for (int i = 0; i < E; ++i) o[i] *= keep;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float f = aw_rescale(a[k].x, M);
-      l += a[k].y * f;
-#pragma unroll
-      for (int i = 0; i < E; ++i) o[i] += x[k][i] * f;
-    }
-  }
-  const float inv = 1.0f / l;
-#pragma unroll
-  for (int i = 0; i < E; ++i) {
-    const float v = o[i] * inv;
-    out[i] = (io_t)(p.gate ? v * sigmoidf_((float)gate[i]) : v);
-  }
-  __builtin_memcpy((io_t*)p.out + oi, out, sizeof out);
-}
-
 }  // namespace trx

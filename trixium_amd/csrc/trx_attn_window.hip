@@ -29,6 +29,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 #include <limits.h>
 
 namespace trx {
@@ -155,6 +156,7 @@ struct AwRing {
     const int u0 = x0 - b.ns + b.lo;
     return x0 >= b.ns && u0 > c.w_last - p.window && u0 <= c.w_first - (kAwKeys - 1);
   }
+  __device__ __forceinline__ static size_t sum_at(const Params&, const Block&, int, size_t at) { return at; }
   template <class Query>
   __device__ __forceinline__ static void queries(const Params&, const Block&, int, int, const Query&, float) {}
   __device__ __forceinline__ static void scored(const Params&, const Block&, int, int, const f32x16_t&, float) {}
@@ -171,6 +173,62 @@ __global__ __launch_bounds__(256, 1) void attn_window_few_kernel(AttnWindowParam
   aw_few<AwRing<HD>, HD, HALF>(p);
 }
 
+// The splits of a (position, head) joined by one wave.
+template <int HD, bool HALF>
+__device__ __forceinline__ void aw_join(const AttnWindowParams& p, int row, int head, int lane) {
+  constexpr int E = HD / 64;                       // dims a lane: E lane .. + E - 1
+  const int g = aw_row(p, head), col = row * p.rep + head - g * p.rep;
+  const size_t all = (size_t)p.nsplit * p.n_kv * p.cols, step = (size_t)p.n_kv * p.cols;
+  const size_t at = (size_t)g * p.cols + col;
+  const float2* ml = (const float2*)((const float*)p.work + all * HD) + at;
+  const float* po = (const float*)p.work + at * HD + E * lane;
+  const size_t gi = (size_t)row * p.gate_stride + (size_t)head * p.gate_head_stride + E * lane;
+  const size_t oi = (size_t)row * p.out_stride + (size_t)head * HD + E * lane;
+  typedef typename std::conditional<HALF, _Float16, float>::type io_t;
+  io_t gate[E], out[E];
+  if (p.gate) __builtin_memcpy(gate, (const io_t*)p.gate + gi, sizeof gate);
+  float M = -INFINITY, l = 0.f, o[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) o[i] = 0.f;
+  // Eight splits' loads at a time in flight (the gate's with them), a running reference over the eights.
+  for (int s0 = 0; s0 < p.nsplit; s0 += 8) {
+    float2 a[8];
+    float x[8][E];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      a[k] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int i = 0; i < E; ++i) x[k][i] = 0.f;
+      if (s0 + k < p.nsplit) {
+        a[k] = ml[(s0 + k) * step];
+        __builtin_memcpy(x[k], po + (s0 + k) * step * HD, 4 * E);
+      }
+    }
+    float top = M;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) top = fmaxf(top, a[k].x);
+    const float keep = aw_rescale(M, top);
+    M = top;
+    l *= keep;
+#pragma unroll
+    for (int i = 0; i < E; ++i) o[i] *= keep;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float f = aw_rescale(a[k].x, M);
+      l += a[k].y * f;
+#pragma unroll
+      for (int i = 0; i < E; ++i) o[i] += x[k][i] * f;
+    }
+  }
+  const float inv = 1.0f / l;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const float v = o[i] * inv;
+    out[i] = (io_t)(p.gate ? v * sigmoidf_((float)gate[i]) : v);
+  }
+  __builtin_memcpy((io_t*)p.out + oi, out, sizeof out);
+}
+
 // After the attention: the splits of each (position, head) joined (a wave each, blocks of four), and
 // the call's last rows of K and V into their slots.
 template <int HD, bool HALF>
@@ -182,8 +240,7 @@ __global__ __launch_bounds__(256) void attn_window_finish(AttnWindowParams p, in
     const unsigned id = blockIdx.x * 4 + w;         // below 2^25 + 4
     if (id >= (unsigned)(p.n * p.n_head)) return;
     const int row = (int)(id / (unsigned)p.n_head);
-    float M, l;
-    aw_join<HD, HALF>(p, row, (int)id - row * p.n_head, lane, M, l);
+    aw_join<HD, HALF>(p, row, (int)id - row * p.n_head, lane);
     return;
   }
   // Rows pos .. pos + n - 1, 16 bytes of K and V a thread. A ring row that a later row of the call
