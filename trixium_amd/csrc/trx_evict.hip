@@ -154,19 +154,19 @@ __global__ __launch_bounds__(kEvThreads) void evict_select_kernel(EvictParams p)
   const int* position = p.positions + (size_t)g * p.slots;
   // Each wave a run of slots, 64 at a time; rows past the last have a key of 0.
   const int rounds = ev_rounds(count), first_u = w * rounds * 64 + lane;
-  // f(slot, key), the lanes of a wave together, from memory, eight rounds' loads in flight; rounds [from, to) of them.
+  // f(slot, key), the lanes of a wave together, from memory, sixteen rounds' loads in flight; rounds [from, to) of them.
   auto read = [&](int from, int to, auto f) AW_INLINE {
-    for (int i = from; i < to; i += 8) {
-      float m[8];
-      int q[8];
+    for (int i = from; i < to; i += 16) {
+      float m[16];
+      int q[16];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < 16; ++k) {
         const int u = min(first_u + 64 * (i + k), count - 1);
         m[k] = mass[u];
         q[k] = position[u];
       }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < 16; ++k) {
         const int u = first_u + 64 * (i + k);
         if (i + k < to) f(u, u < count ? ev_key(p, pos, m[k], q[k]) : 0u);
       }
