@@ -260,9 +260,13 @@ int trx_attn_window(const trx_attn_window_shape* shape, int n, int pos, const in
  * rows of out and its tail stay as they are, as do the rows of out behind a draft's count; their q, k, v and
  * gate may hold anything.
  * kind, head sizes, row strides, alignment and the treatment of infinities and NaN are trx_attn_window's;
- * lengths and counts are 4-byte aligned. prefix <= prefix_slots <= 2^30 (0: kprefix and vprefix may be NULL),
- * 1 <= tail_slots <= 2^30, batch * n * n_head <= 2^23 (batch or n 0: nothing is done). out, workspace and the
- * tails overlap no other argument.
+ * lengths and counts are 4-byte aligned. prefix <= prefix_slots (0: kprefix and vprefix may be NULL), tail_slots >= 1,
+ * both at most 2^30 / n_kv_head, n_head <= 1024, batch * n * n_head <= 2^23 (batch or n 0: nothing is done). out,
+ * workspace and the tails overlap no other argument.
+ * Scores, maxima and sums are fp32. How keys and columns are cut depends on the batch, and with it the last bits of a
+ * draft's outputs; the same call gives the same bits. With TRX_KIND_F16 a prefix under more than 32 columns (batch * n
+ * times the heads of a kv head) and a tail under more than 32 (n times the heads) may also round each probability to
+ * fp16, by 2^-11 of itself.
  * workspace: trx_attn_shared_geometry's bytes, which hold any call of the shape of up to `batch` drafts, `n` new
  * rows and any prefix, no zeroing needed; calls that share it must not overlap. */
 typedef struct trx_attn_shared_shape {
@@ -293,8 +297,11 @@ int trx_attn_shared(const trx_attn_shared_shape* shape, int batch, int n, int pr
  * arguments ignored; values out of range there leave everything as it is.
  * kind, head sizes, row strides, alignment and the treatment of infinities and NaN are trx_attn_window's; mass,
  * positions and state are 4-byte aligned. An infinity or NaN in the query or in a key that it sees may also make
- * the masses of its kv head NaN. slots <= 2^30, n * n_head <= 2^23 (n = 0: nothing is done).
- * Masses do not depend on the order of blocks: the same call gives the same bits.
+ * the masses of its kv head NaN. slots <= 2^30 / n_kv_head, n_head <= 1024, n * n_head <= 2^23 (n = 0: nothing is done).
+ * out, workspace and the cache's arrays overlap no other argument.
+ * Masses are sums in fp32 of probabilities in fp32; they do not depend on the order of blocks: the same call gives the
+ * same bits. With TRX_KIND_F16 calls of more than 32 columns (n times the heads of a kv head) may round each
+ * probability to fp16 in the outputs, by 2^-11 of itself.
  * workspace: trx_attn_mass_geometry's bytes for n, which hold any call of the shape of up to n positions, no
  * zeroing needed; calls that share it must not overlap.
  *

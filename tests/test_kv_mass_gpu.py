@@ -146,7 +146,7 @@ def evict_geometry(shape):
 
 @pytest.mark.parametrize("change,what", [
     (dict(head_dim=96), b"head_dim"), (dict(n_kv_head=0), b"n_head"), (dict(n_head=5), b"n_head"), (dict(slots=0), b"slots"),
-    (dict(slots=(1 << 30) + 1), b"slots"), (dict(scale=-1.0), b"scale"), (dict(q_stride=252), b"q_stride"),
+    (dict(slots=(1 << 30) + 1), b"slots"), (dict(slots=(1 << 29) + 1), b"slots"), (dict(scale=-1.0), b"scale"), (dict(q_stride=252), b"q_stride"),
     (dict(q_stride=258), b"q_stride"), (dict(kv_stride=132), b"kv_stride"), (dict(out_stride=255), b"out_stride"),
     (dict(kind=L.KIND_Q8), b"kind")])
 def test_geometry_refuses(change, what):

@@ -136,7 +136,8 @@ def geometry(shape, batch, n, prefix):
     (dict(head_dim=96), b"head_dim"), (dict(n_kv_head=0), b"n_head"), (dict(n_head=5), b"n_head"),
     (dict(n_head=2048, q_stride=2048 * 64, out_stride=2048 * 64), b"heads"),
     (dict(prefix_slots=-1), b"slots"), (dict(prefix_slots=(1 << 30) + 1), b"slots"), (dict(tail_slots=0), b"slots"),
-    (dict(tail_slots=(1 << 30) + 1), b"slots"), (dict(prefix_slots=39), b"prefix"), (dict(scale=0.0), b"scale"),
+    (dict(tail_slots=(1 << 30) + 1), b"slots"), (dict(tail_slots=(1 << 29) + 1), b"slots"),
+    (dict(prefix_slots=(1 << 29) + 1), b"slots"), (dict(prefix_slots=39), b"prefix"), (dict(scale=0.0), b"scale"),
     (dict(scale=float("nan")), b"scale"), (dict(scale=float("inf")), b"scale"), (dict(q_stride=252), b"q_stride"),
     (dict(q_stride=258), b"q_stride"), (dict(kv_stride=132), b"kv_stride"), (dict(kv_stride=(1 << 22) + 8), b"kv_stride"),
     (dict(out_stride=255), b"out_stride"), (dict(kind=L.KIND_Q8), b"kind")])

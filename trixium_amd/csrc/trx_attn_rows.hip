@@ -342,8 +342,14 @@ __global__ __launch_bounds__(256) void attn_rows_finish(AttnRowsParams p, int ma
 }
 
 // Many columns: the scores once more, with the keys' rows in registers (KT tiles of 32 a wave) while the columns pass
-// through LDS, 32 for each of CG groups of KW waves a stage; a lane adds up its column's probabilities of its keys,
-// lanes and groups are added at the end. The queries come as the attention left them, in operands' order.
+// through LDS, 32 for each of CG groups of KW waves a step; a lane adds up its column's probabilities of its keys,
+// lanes and groups are added at the end. (Columns that stayed while the keys passed would have to add up each key over
+// the lanes.) The queries come as the attention left them, in operands' order, so that a step's bytes come straight
+// into LDS and are read in a row. Eight waves, two a SIMD: the matrix instructions of one run beside the exponentials
+// of both. Of 1024 fp32 positions of 32 heads of 128 over 2900 rows 66 us, 0.87 PFLOP/s with both planes counted, of
+// 1021 fp16 ones over 7001 rows 94 us (four matrix instructions take a SIMD 66 ns, so that 28 and 31 us would be all of
+// them without a pause); without the loads 9 and 12 us less. Scores and exponentials one after the other took 80 and
+// 115, masks in the loop 71 and 96.
 template <int HD, bool HALF>
 struct ArMass {
   static constexpr int KT = HD == 256 ? 1 : 2, KW = HD == 256 ? 4 : 2, CG = 8 / KW;
@@ -510,7 +516,15 @@ static int ar_most_rows(const AttnRowsParams& p) { return p.state || p.lengths ?
 
 // What a cut of a segment takes by this estimate, in microseconds, with `others` blocks beside it: a block takes a fixed
 // part (its queries, the first rows' latency, the join of its waves, the outputs) and a step for each wk tiles of keys;
-// a full chip makes a step 1.4 times as long.
+// a full chip makes a step 1.4 times as long. Measured (us; waves of columns and splits of the prefix, splits of the
+// tails), the choice first:
+//   24 drafts over 4001 rows and up to 300 of their own, 32 heads of 128, 8 kv heads: (1, 12; 1) 20; (1, 8; 1) 20,
+//     (1, 4; 1) 25, (1, 16; 2) 27, (4, 32; 1) 35
+//   64 over 32768 and up to 999, fp16: (4, 16; 1) 93; (4, 8; 1) 106, (2, 8; 1) 109, (4, 24; 1) 109, (1, 8; 1) 130
+//   12 of 7 rows over 6001 and up to 200, fp16: (4, 10; 2) 35; (4, 8; 2) 36, (2, 4; 2) 36, (1, 8; 1) 39, (4, 16; 2) 44
+//   8 over 2047 and up to 130, 24 heads of 256, 4 kv heads: (1, 16; 2) 20; (1, 8; 1) 23, (2, 16; 1) 39
+//   one token with masses over 32700, fp16: 32 splits 38; 24 41, 64 41, 48 43, 16 49
+//   27 with masses over 1900, 24 heads of 256: (1, 8) 37; (1, 6) 41, (1, 4) 44, (1, 12) 54, (2, 16) 64
 static double ar_time(const AttnRowsParams& p, const ArCut& c, int units, int cols, int keys, long long others) {
   const int wk = c.wq == 1 ? 4 : (p.hd == 256 ? 4 : 8) / c.wq;
   const double fixed = c.wq == 1 ? 2 : 11;
@@ -535,7 +549,8 @@ static void ar_plan(const AttnRowsParams& p, ArCut& prefix, ArCut& tail) {
   const int rep = p.n_head / p.n_kv, cols = p.n * rep, all = p.batch * cols, keys = ar_most_rows(p);
   const long long rows = (long long)p.batch * p.n * p.n_head;
   const double part = 8.0 * rows * p.hd / 6e6;       // a part of every column written and read, at 6 TB/s
-  // Each segment alone, one launch behind the other (a prefix brings the join with it).
+  // Each segment alone, one launch behind the other (a prefix brings the join with it). Up to 32 columns stay with the
+  // kernel for few: wide blocks would leave most of theirs empty, and round fp16's probabilities for it.
   double time = 0, least = 1e300;
   for (int wq : {1, 2, 4}) {
     if (wq > 1 && cols <= 32) break;
@@ -548,11 +563,13 @@ static void ar_plan(const AttnRowsParams& p, ArCut& prefix, ArCut& tail) {
   if (p.prefix > 0) {
     time = least + 2;
     least = 1e300;
-    for (int wq : {1, 2, 4})
+    for (int wq : {1, 2, 4}) {
+      if (wq > 1 && all <= 32) break;
       ar_cuts(wq, p.prefix, rows, [&](const ArCut& c) {
         const double t = ar_time(p, c, 1, all, p.prefix, 0) + c.splits * part;
         if (t < least) least = t, prefix = c;
       });
+    }
     time += least;
     // Both in one launch, of few columns a block.
     ar_cuts(1, keys, rows, [&](const ArCut& b) {
@@ -572,6 +589,8 @@ const char* attn_rows_refuses(const AttnRowsParams& p) {
   if (p.n_kv < 1 || p.n_head < 1 || p.n_head % p.n_kv) return "n_head is not a multiple of n_kv_head";
   if (p.n_head > 1024) return "more than 1024 heads";
   if (p.prefix_slots < 0 || p.prefix_slots > 1 << 30 || p.tail_slots < 1 || p.tail_slots > 1 << 30) return "slots outside [1, 2^30]";
+  // (The masses' blocks, of 128 keys, stay below a grid's 2^32 threads.)
+  if ((long long)p.tail_slots * p.n_kv > 1 << 30 || (long long)p.prefix_slots * p.n_kv > 1 << 30) return "more than 2^30 slots of all kv heads";
   if (p.prefix < 0 || p.prefix > p.prefix_slots) return "prefix outside [0, prefix_slots]";
   // (Blocks of 256 threads, one a column at most, stay below a grid's 2^32 threads.)
   if (p.batch < 0 || p.n < 0 || (p.batch > 0 && (long long)p.n * p.n_head > (1 << 23) / p.batch)) return "too many rows";
