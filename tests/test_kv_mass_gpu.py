@@ -428,6 +428,26 @@ def test_one_workspace_for_a_prompt_and_its_rest():
         assert (work.download(np.uint8, guard, offset=size) == 0xA5).all(), n
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,hd,n", [(32, 8, 128, 1), (6, 1, 256, 5), (4, 2, 64, 9), (8, 8, 128, 31)])
+def test_few_columns_with_fp16_queries_round_once(heads, kv, hd, n):
+    """As test_shared_prefix_gpu.py's: up to 32 columns' fp16 outputs are the fp32 result rounded."""
+    c = Cache(heads, kv, hd, 1500 + n, F16, seed=16, scale=1.0)
+    q, k, v = c.rows(n)
+    q[..., 1:] = 0
+    out, *_ = c.attend(q, k, v, 1500, 1500)
+    out = out.reshape(n, heads, hd).astype(np.float64)
+    K, V = (np.concatenate([a[:, :1500], x.transpose(1, 0, 2)], axis=1).astype(np.float64) for a, x in ((c.K, k), (c.V, v)))
+    for r in range(n):
+        for h in range(heads):
+            g, N = h * kv // heads, 1500 + r + 1
+            s = K[g, :N, 0] * float(q[r, h, 0])
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            x, d = p @ V[g, :N], (p @ np.abs(V[g, :N])) * (2 * (np.abs(s).max() + 1) * 2.0**-21 + N * 2.0**-24 + 2.0**-22)
+            assert (np.abs(out[r, h] - x) <= np.abs(x.astype(np.float16).astype(np.float64) - x) + 2 * d).all(), (r, h)
+
+
 # Eviction (GPU) -------------------------------------------------------------------------------------------
 
 

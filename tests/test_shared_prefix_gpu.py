@@ -479,3 +479,55 @@ def test_shared_prefix_object():
         d.attend(np.zeros((4, 40, 4, 64)), np.zeros((4, 40, 2, 64)), np.zeros((4, 40, 2, 64)))     # past the slots
     with pytest.raises(ValueError):
         d.cut([9] * 4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,hd,batch,n", [(32, 8, 128, 8, 1), (6, 1, 256, 5, 1), (4, 2, 64, 4, 4), (8, 8, 128, 3, 5)])
+def test_few_columns_with_fp16_queries_round_once(heads, kv, hd, batch, n):
+    """Up to 32 columns' fp16 outputs are the fp32 result rounded: x + d rounds to a value whose distance from x is at most
+    that of x rounded, plus 2 d. Queries with one element leave a score no sum over dims: d is the fp32 tolerance
+    without it."""
+    c = Drafts(heads, kv, hd, batch, 1900, 60, F16, seed=15, scale=1.0)
+    q, k, v = c.rows(n)
+    q[..., 1:] = 0
+    lengths = c.rng.integers(0, 60 - n + 1, batch)
+    out, _, _ = c.call(q, k, v, lengths)
+    out = out.reshape(batch * n, heads, hd).astype(np.float64)
+    for r in range(batch * n):
+        b, i = divmod(r, n)
+        K, V = (np.concatenate([p, t[b][:, :lengths[b]], x[b * n:b * n + i + 1].transpose(1, 0, 2)], axis=1).astype(np.float64)
+                for p, t, x in ((c.kp, c.kt, k), (c.vp, c.vt, v)))
+        for h in range(heads):
+            g = h * kv // heads
+            s = K[g, :, 0] * float(q[r, h, 0])
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            x, d = p @ V[g], (p @ np.abs(V[g])) * (2 * (np.abs(s).max() + 1) * 2.0**-21 + s.size * 2.0**-24 + 2.0**-22)
+            assert (np.abs(out[r, h] - x) <= np.abs(x.astype(np.float16).astype(np.float64) - x) + 2 * d).all(), (r, h)
+
+
+@pytest.mark.gpu
+def test_two_calls_at_once():
+    """Two batches over one prefix on streams of their own, each with its workspace: the bits of each alone."""
+    c = Drafts(32, 8, 128, 12, 3000, 90, seed=16)
+    B, shape = _lib.DeviceBuffer, c.shape()
+    calls = []
+    kp, vp = B.from_array(c.kp), B.from_array(c.vp)
+    for _ in range(2):
+        q, k, v = c.rows(2)
+        lengths = c.rng.integers(0, 89, 12)
+        want = c.call(q, k, v, lengths)
+        s = ctypes.c_void_p()
+        _lib.call("trx_stream_create", ctypes.byref(s))
+        bufs = [B.from_array(a) for a in (lengths.astype(np.int32), q, k, v, c.kt, c.vt)]
+        calls.append((want, s, bufs, B(q.nbytes), B(geometry(shape, 12, 2, 3000))))
+    _lib.synchronize()
+    for _ in range(3):
+        for want, s, (lb, qb, kb, vb, kt, vt), out, work in calls:
+            _lib.call("trx_attn_shared", ctypes.byref(shape), 12, 2, 3000, lb.ptr, None, qb.ptr, kb.ptr, vb.ptr, kp.ptr, vp.ptr,
+                      kt.ptr, vt.ptr, None, out.ptr, work.ptr, s)
+        for want, s, bufs, out, work in calls:
+            _lib.synchronize(s)
+            assert np.array_equal(out.download(np.uint8, out.nbytes), want[0].view(np.uint8).ravel())
+    for _, s, *_ in calls:
+        _lib.call("trx_stream_destroy", s)
