@@ -92,7 +92,7 @@ struct ArRows {
 };
 
 // Rows in a line as a layout of the keys (trx_attn_tile.h).
-template <int HD, bool MASS>
+template <int HD, bool HALF, bool MASS>
 struct ArLine {
   using Params = AttnRowsParams;
   using Block = ArBlock;
@@ -151,18 +151,16 @@ struct ArLine {
   __device__ __forceinline__ static size_t sum_at(const Params& p, const Block& b, int col, size_t) {
     return ((size_t)b.g * p.cols + col) * p.nsplit + b.sp;
   }
-  // Queries as the mass kernel takes them: a wave's 32 columns, plane by plane, chunk by chunk, 16 bytes a lane.
-  template <class Query>
-  __device__ __forceinline__ static void queries(const Params& p, const Block& b, int first, int lane, const Query& q, float cs) {
+  // Chunk k of a wave's 32 queries as the mass kernel takes them: column block by column block, plane by plane, 16 bytes
+  // a lane.
+  __device__ __forceinline__ static void query(const Params& p, const Block& b, int first, int lane, int k, const half8_t& hi,
+                                               const half8_t& lo, float cs) {
     if (!MASS || !p.planes || b.split || first >= p.cols) return;
-    constexpr int NC = HD / 16, ALL = NC + (sizeof(q.lo) > sizeof(half8_t) ? NC : 0);
+    constexpr int NC = HD / 16, ALL = HALF ? NC : 2 * NC;
     half8_t* to = (half8_t*)p.planes + ((size_t)b.g * ((p.cols + 31) / 32) + first / 32) * ALL * 64 + lane;
-#pragma unroll
-    for (int k = 0; k < NC; ++k) {
-      to[k * 64] = q.hi[k];
-      if constexpr (ALL > NC) to[(NC + k) * 64] = q.lo[k];
-    }
-    if (lane < 32 && first + lane < p.cols) p.norms[(size_t)b.g * p.cols + first + lane].z = cs;
+    to[k * 64] = hi;
+    if constexpr (!HALF) to[(NC + k) * 64] = lo;
+    if (k == 0 && lane < 32 && first + lane < p.cols) p.norms[(size_t)b.g * p.cols + first + lane].z = cs;
   }
   // A lane's scores of keys x, x + 8, x + 16 and x + 24, four each, in powers of two.
   __device__ __forceinline__ static void scored(const Params& p, const Block& b, int col, int x, const f32x16_t& s, float cs) {
@@ -182,7 +180,7 @@ struct ArLine {
 // 1024 fp32 positions over 2900 rows 130 us, 0.88 with both planes counted; bound as the window attention's chunks.
 template <int HD, bool HALF, bool MASS, int WQ, int WK, int D>
 __global__ __launch_bounds__(64 * WQ * WK, WQ * WK / 4) void attn_rows_kernel(AttnRowsParams p) {
-  aw_many<ArLine<HD, MASS>, HD, HALF, WQ, WK, D>(p);
+  aw_many<ArLine<HD, HALF, MASS>, HD, HALF, WQ, WK, D>(p);
 }
 
 // Few columns (aw_few): one token over 32700 rows (134 MB) 33 us, 4.1 TB/s, 30 without keeping the scores; the tails of 64
@@ -190,7 +188,7 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ * WK / 4) void attn_rows_kernel(At
 // drafts over 4001 rows 20 us in all, 24 with one block a CU, where the token is as fast.
 template <int HD, bool HALF, bool MASS>
 __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attn_rows_few_kernel(AttnRowsParams p) {
-  aw_few<ArLine<HD, MASS>, HD, HALF>(p);
+  aw_few<ArLine<HD, HALF, MASS>, HD, HALF>(p);
 }
 
 // The parts of a (row, head) joined by one wave: a lane has the reference and the sum of parts lane and lane + 64, so

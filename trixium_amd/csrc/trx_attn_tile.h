@@ -9,7 +9,7 @@
 //     0 .. N - 1; split of splits, its share of them, and sp, the part that its sums are;
 //   Rows: the places of the keys' rows (row, flat); Column: row, head and the columns it stands with;
 //   block (false: nothing to do), sight (whether a column sees a key), whole (stages that every column of a wave
-//     sees whole), all_see (one tile); and what a layout may keep of the work: queries (a wave's, as operands),
+//     sees whole), all_see (one tile); and what a layout may keep of the work: query (a chunk of a wave's, as operands),
 //     scored (a tile's scores, in calls of few columns), total (of a column that one block finishes: its maximum and
 //     sum).
 #pragma once
@@ -115,49 +115,59 @@ __device__ __forceinline__ int aw_share(int count, int split, int splits) {
 template <int HD, bool HALF>
 struct AwQuery {
   static constexpr int NC = HD / 16;
+  typedef float f32x4_t __attribute__((ext_vector_type(4)));
   half8_t hi[NC], lo[HALF ? 1 : NC];
 
-  // piece(i): 16 bytes of the lane's query, from element (HALF ? 8 : 4) i on. Returns the powers of two per
-  // unit of raw score.
+  // piece(i): 16 bytes of the lane's query, from element (HALF ? 8 : 4) i on. The powers of two per unit of raw score,
+  // and what the elements are multiplied by before they are rounded.
+  template <class Piece>
+  __device__ __forceinline__ static float unit(float scale, int h, Piece piece, float& up) {
+    const float cs = scale * kLog2e;
+    up = 1.f;
+    if constexpr (HALF) return cs;
+    float amax = 0.f;
+#pragma unroll
+    for (int k = 0; k < NC; ++k)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const f32x4_t a = __builtin_bit_cast(f32x4_t, piece(4 * k + 2 * h + i));
+        amax = fmaxf(amax, fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))));
+      }
+    amax = both_halves_max(amax);
+    int e = 0;
+    if (amax > 0.f && amax < INFINITY) {
+      frexpf(amax, &e);                           // amax < 2^e
+      e = min(max(14 - e, -114), 100);
+    }
+    up = ldexpf(1.f, e);
+    return ldexpf(cs, -e);
+  }
+  // Chunk k of both planes.
+  template <class Piece>
+  __device__ __forceinline__ static void chunk(int k, int h, float up, Piece piece, half8_t& hi, half8_t& lo) {
+    if constexpr (HALF) {
+      hi = __builtin_bit_cast(half8_t, piece(2 * k + h));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const f32x4_t a = __builtin_bit_cast(f32x4_t, piece(4 * k + 2 * h + i));
+#pragma unroll
+        for (int l = 0; l < 4; ++l) {
+          const float x = a[l] * up;
+          const _Float16 top = (_Float16)x;
+          hi[4 * i + l] = top;
+          lo[4 * i + l] = (_Float16)(x - (float)top);
+        }
+      }
+    }
+  }
   template <class Piece>
   __device__ __forceinline__ float take(float scale, int h, Piece piece) {
-    const float cs = scale * kLog2e;
-    if constexpr (HALF) {
+    float up;
+    const float cs = unit(scale, h, piece, up);
 #pragma unroll
-      for (int k = 0; k < NC; ++k) hi[k] = __builtin_bit_cast(half8_t, piece(2 * k + h));
-      return cs;
-    } else {
-      typedef float f32x4_t __attribute__((ext_vector_type(4)));
-      float amax = 0.f;
-#pragma unroll
-      for (int k = 0; k < NC; ++k)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const f32x4_t a = __builtin_bit_cast(f32x4_t, piece(4 * k + 2 * h + i));
-          amax = fmaxf(amax, fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))));
-        }
-      amax = both_halves_max(amax);
-      int e = 0;
-      if (amax > 0.f && amax < INFINITY) {
-        frexpf(amax, &e);                         // amax < 2^e
-        e = min(max(14 - e, -114), 100);
-      }
-      const float up = ldexpf(1.f, e);
-#pragma unroll
-      for (int k = 0; k < NC; ++k)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const f32x4_t a = __builtin_bit_cast(f32x4_t, piece(4 * k + 2 * h + i));
-#pragma unroll
-          for (int l = 0; l < 4; ++l) {
-            const float x = a[l] * up;
-            const _Float16 top = (_Float16)x;
-            hi[k][4 * i + l] = top;
-            lo[k][4 * i + l] = (_Float16)(x - (float)top);
-          }
-        }
-      return ldexpf(cs, -e);
-    }
+    for (int k = 0; k < NC; ++k) chunk(k, h, up, piece, hi[k], lo[HALF ? 0 : k]);
+    return cs;
   }
 };
 
@@ -515,7 +525,10 @@ __device__ __forceinline__ void aw_many(const typename Layout::Params& p) {
     wait_loads_and_block<0>();
     const uint32_t mine = ks + (32 * wq + j) * QROW;
     v.init(q.take(p.scale, h, [&](int i) { return __builtin_bit_cast(u32x4_t, lds_half8(mine + 16 * (i ^ swizzle(j)))); }));
-    if (wk == 0) Layout::queries(p, b, b.c0 + 32 * wq, lane, q, v.cs);
+    if (wk == 0) {
+#pragma unroll
+      for (int k = 0; k < HD / 16; ++k) Layout::query(p, b, b.c0 + 32 * wq, lane, k, q.hi[k], q.lo[HALF ? 0 : k], v.cs);
+    }
     wait_loads_and_block<0>();
   }
 
@@ -730,16 +743,21 @@ __device__ __forceinline__ void aw_few(const typename Layout::Params& p) {
   wait_loads_and_block<0>();
   Wave v;
   {
-    AwQuery<HD, HALF> q;
+    // (Each wave a share of the chunks: all of them by every wave took 1 us with 256 dims.)
+    using Query = AwQuery<HD, HALF>;
     const uint32_t at = lds_address(smem) + mine * QROW;
-    v.init(q.take(p.scale, h, [&](int i) { return __builtin_bit_cast(u32x4_t, lds_half8(at + 16 * (i ^ swizzle(mine)))); }));
-    if (wk == 0) Layout::queries(p, b, b.c0, lane, q, v.cs);
+    auto piece = [&](int i) AW_INLINE { return __builtin_bit_cast(u32x4_t, lds_half8(at + 16 * (i ^ swizzle(mine)))); };
+    float up;
+    v.init(Query::unit(p.scale, h, piece, up));
 #pragma unroll
-    for (int k = 0; k < Wave::NC; ++k)
-      if (k % WK == wk) {
-        *(half8_t*)(qs + j * QS + 16 * k + 8 * h) = q.hi[k];
-        if constexpr (!HALF) *(half8_t*)(qs + 32 * QS + j * QS + 16 * k + 8 * h) = q.lo[k];
-      }
+    for (int i = 0; i < Wave::NC / WK; ++i) {
+      const int k = WK * i + wk;
+      half8_t hi, lo;
+      Query::chunk(k, h, up, piece, hi, lo);
+      *(half8_t*)(qs + j * QS + 16 * k + 8 * h) = hi;
+      if constexpr (!HALF) *(half8_t*)(qs + 32 * QS + j * QS + 16 * k + 8 * h) = lo;
+      Layout::query(p, b, b.c0, lane, k, hi, lo, v.cs);
+    }
   }
   __syncthreads();
   const _Float16* const qr = qs + j * QS + 8 * h;

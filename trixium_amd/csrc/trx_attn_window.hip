@@ -157,8 +157,7 @@ struct AwRing {
     return x0 >= b.ns && u0 > c.w_last - p.window && u0 <= c.w_first - (kAwKeys - 1);
   }
   __device__ __forceinline__ static size_t sum_at(const Params&, const Block&, int, size_t at) { return at; }
-  template <class Query>
-  __device__ __forceinline__ static void queries(const Params&, const Block&, int, int, const Query&, float) {}
+  __device__ __forceinline__ static void query(const Params&, const Block&, int, int, int, const half8_t&, const half8_t&, float) {}
   __device__ __forceinline__ static void scored(const Params&, const Block&, int, int, const f32x16_t&, float) {}
   __device__ __forceinline__ static void total(const Params&, const Block&, int, const float2&) {}
 };
