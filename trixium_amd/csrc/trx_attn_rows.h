@@ -39,7 +39,7 @@ struct AttnRowsParams {
   int prefix_splits, tail_splits;
   int prefix_blocks;           // of this launch, before the tails' blocks
   int prefix_cb, tail_cb;      // column blocks of the batch and of a draft
-  float* scores;               // [n_kv][cols][score_ld], powers of two, of calls of few columns with masses
+  float* scores;               // [n_kv][cols][score_ld], powers of two, of calls with masses that keep them
   long long score_ld;
   float4* norms;               // [n_kv][cols]: a probability is 2^(z raw score - x) y
   void* planes;                // the queries as operands, of calls of many columns with masses

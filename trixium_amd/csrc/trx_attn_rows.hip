@@ -307,18 +307,67 @@ __device__ __forceinline__ void ar_mass_few(const AttnRowsParams& p, int block, 
   }
 }
 
+// Up to 256 columns: the masses of 64 keys a block, each wave a quarter of the columns, the columns' parts joined by a thread
+// each. A block of columns has left scores of the keys that it sees alone.
+constexpr int kArMassColumns = 256;
+__device__ __forceinline__ void ar_mass_some(const AttnRowsParams& p, int block, float2* norm, float* part) {
+  const int kb = block / p.n_kv, g = block - kb * p.n_kv, lane = threadIdx.x & 63, w = threadIdx.x >> 6, x = kb * 64 + lane;
+  int have, fresh;
+  if (!ar_sequence(p, 0, have, fresh)) return;
+  const int N = have + fresh, c = threadIdx.x;
+  if (kb * 64 >= N) return;
+  if (c < p.cols) {
+    if (p.nsplit > 1) {
+      const size_t all = (size_t)p.nsplit * p.n_kv * p.cols;
+      const float2* ml = (const float2*)((const float*)p.work + all * p.hd) + ((size_t)g * p.cols + c) * p.nsplit;
+      float M = -INFINITY, l = 0.f;
+      for (int s0 = 0; s0 < p.nsplit; s0 += 8) {
+        float2 a[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) a[k] = s0 + k < p.nsplit ? ml[s0 + k] : make_float2(-INFINITY, 0.f);
+        float to = M;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) to = fmaxf(to, a[k].x);
+        l *= aw_rescale(M, to);
+        M = to;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) l += a[k].y * aw_rescale(a[k].x, M);
+      }
+      norm[c] = ar_norm(M, l);
+    } else {
+      norm[c] = *(const float2*)(p.norms + (size_t)g * p.cols + c);
+    }
+  }
+  __syncthreads();
+  const float* s = p.scores + (size_t)g * p.cols * p.score_ld + min(x, p.tail_slots - 1);
+  float sum = 0.f;
+#pragma unroll 8
+  for (int i = w; i < p.cols; i += 4) {
+    const float e = fmaf(__builtin_amdgcn_exp2f(s[i * p.score_ld] - norm[i].x), norm[i].y, sum);
+    sum = x <= have + aw_row(p, i) ? e : sum;
+  }
+  part[64 * w + lane] = sum;
+  __syncthreads();
+  if (w || x >= N) return;
+  sum = part[lane] + part[64 + lane] + part[128 + lane] + part[192 + lane];
+  float* m = p.mass + (size_t)g * p.tail_slots + x;
+  *m = x < have ? *m + sum : sum;
+}
+
 // After the attention: the parts of each (row, head) joined (a wave each, blocks of four), the new rows into the
 // tails' slots, and the masses of calls of few columns. Bound by latency: 13 parts of 24 drafts 4 us, 17 of 64 drafts 7 (18
 // MB of parts), one token's 32 parts and 32700 masses of 8 kv heads 6.
 template <int HD, bool HALF, bool MASS>
 __global__ __launch_bounds__(256) void attn_rows_finish(AttnRowsParams p, int mass_blocks, int join_blocks) {
-  __shared__ float2 norm[32];
+  __shared__ float2 norm[MASS ? kArMassColumns : 1];
+  __shared__ float part[MASS ? 256 : 1];
   int pos = 0;
   if (MASS && !ar_position(p, pos)) return;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   // (First, so that a kv head's masses are added up on the XCD that has its scores.)
   if (MASS && (int)blockIdx.x < mass_blocks) {
-    ar_mass_few(p, blockIdx.x, norm);
+    if (p.cols <= 32) ar_mass_few(p, blockIdx.x, norm);
+    else ar_mass_some(p, blockIdx.x, norm, part);
     return;
   }
   const int block = (int)blockIdx.x - mass_blocks;
@@ -528,7 +577,7 @@ static int ar_most_rows(const AttnRowsParams& p) { return p.state || p.lengths ?
 //   12 of 7 rows over 6001 and up to 200, fp16: (4, 10; 2) 35; (4, 8; 2) 36, (2, 4; 2) 36, (1, 8; 1) 39, (4, 16; 2) 44
 //   8 over 2047 and up to 130, 24 heads of 256, 4 kv heads: (1, 16; 2) 20; (1, 8; 1) 23, (2, 16; 1) 39
 //   one token with masses over 32700, fp16: 32 splits 38; 24 41, 64 41, 48 43, 16 49
-//   27 with masses over 1900, 24 heads of 256: (1, 8) 37; (1, 6) 41, (1, 4) 44, (1, 12) 54, (2, 16) 64
+//   27 with masses over 1900, 24 heads of 256: (1, 8) 27; (1, 10) 27, (1, 6) 30, (1, 4) 35, (2, 16) 41, (1, 12) 42
 static double ar_time(const AttnRowsParams& p, const ArCut& c, int units, int cols, int keys, long long others) {
   const int wk = c.wq == 1 ? 4 : (p.hd == 256 ? 4 : 8) / c.wq;
   const double fixed = c.wq == 1 ? 2 : 11;
@@ -610,7 +659,14 @@ const char* attn_rows_refuses(const AttnRowsParams& p) {
 }
 
 static long long ar_score_ld(const AttnRowsParams& p) { return ((long long)p.tail_slots + 31) / 32 * 32; }
-static bool ar_few(const AttnRowsParams& p) { return p.n * (p.n_head / p.n_kv) <= 32; }
+// Scores are kept of up to 32 columns, however long the cache, and of up to 256 in 16 MB. (27 positions of 24 heads of 256 over
+// 1900 rows, 5 MB: 27 us, 36 where they are taken again; of 32 heads of 128 over 4000, 14 MB: 26 and 31; 60 of them, 31 MB: 41
+// and 41.)
+constexpr size_t kArScoreBytes = 16 << 20;
+static bool ar_keeps(const AttnRowsParams& p, const ArCut& tail) {
+  const int cols = p.n * (p.n_head / p.n_kv);
+  return cols <= 32 || (tail.wq == 1 && cols <= kArMassColumns && (size_t)cols * p.n_kv * ar_score_ld(p) * 4 <= kArScoreBytes);
+}
 
 // Parts of the prefix and of the tails: one split of each, or as many as kArPartRows allows.
 static size_t ar_parts_bytes(const AttnRowsParams& p) {
@@ -618,8 +674,8 @@ static size_t ar_parts_bytes(const AttnRowsParams& p) {
   return (size_t)(2 * std::min(std::max<long long>(rows, kArPartRows), kArMaxSplits * rows)) * (p.hd + 2) * 4;
 }
 static size_t ar_score_bytes(const AttnRowsParams& p) {
-  const int rep = p.n_head / p.n_kv;
-  return (size_t)std::min(p.n * rep, 32) * p.n_kv * ar_score_ld(p) * 4;
+  const size_t column = (size_t)p.n_kv * ar_score_ld(p) * 4, cols = (size_t)p.n * (p.n_head / p.n_kv);
+  return std::max(std::min<size_t>(cols, 32) * column, std::min(cols * column, kArScoreBytes));
 }
 size_t attn_rows_work_bytes(const AttnRowsParams& p) { return ar_parts_bytes(p); }
 static size_t ar_norm_bytes(const AttnRowsParams& p) { return (size_t)p.n * p.n_head * sizeof(float4); }
@@ -652,7 +708,7 @@ static int ar_launch(AttnRowsParams& p, const ArCut& prefix, const ArCut& tail, 
   TRX_LAUNCHED();
   const int join = p.nsplit > 1 ? (int)(((long long)p.batch * p.n * p.n_head + 3) / 4) : 0;
   const int append = (int)(((long long)p.batch * p.n * p.n_kv * (HD / 8) + 255) / 256);
-  const int masses = p.scores ? cdiv(ar_most_rows(p), kArMassKeys) * p.n_kv : 0;
+  const int masses = p.scores ? cdiv(ar_most_rows(p), p.cols <= 32 ? kArMassKeys : 64) * p.n_kv : 0;
   hipLaunchKernelGGL((attn_rows_finish<HD, HALF, MASS>), dim3(masses + join + append), dim3(256), 0, s, p, masses, join);
   TRX_LAUNCHED();
   if constexpr (MASS) {
@@ -686,10 +742,11 @@ int launch_attn_rows(const AttnRowsParams& params, hipStream_t s) {
   p.nsplit = prefix.splits + tail.splits;
   if (p.mass) {
     char* at = (char*)p.work + ar_parts_bytes(p);
-    p.scores = ar_few(p) ? (float*)at : nullptr;
+    const bool keeps = ar_keeps(p, tail);
+    p.scores = keeps ? (float*)at : nullptr;
     p.score_ld = ar_score_ld(p);
     p.norms = (float4*)(at + ar_score_bytes(p));
-    p.planes = ar_few(p) ? nullptr : at + ar_score_bytes(p) + ar_norm_bytes(p);
+    p.planes = keeps ? nullptr : at + ar_score_bytes(p) + ar_norm_bytes(p);
   }
   if (p.half_io) {
     if (p.hd == 64) return ar_launch<64, true>(p, prefix, tail, s);
