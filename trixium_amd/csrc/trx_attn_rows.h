@@ -42,6 +42,7 @@ struct AttnRowsParams {
   float* scores;               // [n_kv][cols][score_ld], powers of two, of calls with masses that keep them
   long long score_ld;
   float4* norms;               // [n_kv][cols]: a probability is 2^(z raw score - x) y
+  float* partial;              // [parts][kv head and block of keys][128], sums of a part of the columns
   void* planes;                // the queries as operands, of calls of many columns with masses
 };
 

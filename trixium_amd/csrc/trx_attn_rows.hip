@@ -403,11 +403,13 @@ __global__ __launch_bounds__(256) void attn_rows_finish(AttnRowsParams p, int ma
 // 1021 fp16 ones over 7001 rows 94 us (four matrix instructions take a SIMD 66 ns, so that 28 and 31 us would be all of
 // them without a pause); without the loads 9 and 12 us less. Scores and exponentials one after the other took 80 and
 // 115, masks in the loop 71 and 96.
+constexpr int kArMassBlock = 128;                   // keys
 template <int HD, bool HALF>
 struct ArMass {
   static constexpr int KT = HD == 256 ? 1 : 2, KW = HD == 256 ? 4 : 2, CG = 8 / KW;
   static constexpr int KEYS = 32 * KT * KW;                    // a block's
   static constexpr int NC = HD / 16, ALL = HALF ? NC : 2 * NC;  // KB of 32 columns' operands
+  static_assert(KEYS == kArMassBlock, "the parts' layout");
   static constexpr int SB = HALF ? 2 : 1;                      // steps of CG column blocks a stage
   static constexpr int B = SB * CG * ALL * 1024;               // bytes of a stage
 };
@@ -438,15 +440,18 @@ __global__ __launch_bounds__(512, 2) void attn_mass_kernel(AttnRowsParams p) {
 #pragma unroll
     for (int k = 0; k < A::NC; ++k) kf[t][k] = *(const half8_t*)(kr + 32 * k);
   }
-  // Columns before the first new row that sees the block's first key have nothing for it.
-  const int cbs = (p.cols + 31) / 32, cb0 = max(0, kb * A::KEYS - b.cached) * p.rep / 32;
+  // Columns before the first new row that sees the block's first key have nothing for it; the steps over the others are
+  // shared by the parts.
+  const int cbs = (p.cols + 31) / 32, from0 = max(0, kb * A::KEYS - b.cached) * p.rep / 32;
+  const int every = (cbs - from0 + A::CG - 1) / A::CG, step0 = aw_share(every, blockIdx.y, gridDim.y);
+  const int cb0 = from0 + step0 * A::CG, steps = aw_share(every, blockIdx.y + 1, gridDim.y) - step0;
   const char* planes = (const char*)p.planes + (size_t)b.g * cbs * A::ALL * 1024;
   const float4* norms = p.norms + (size_t)b.g * p.cols;
   const uint32_t lds = lds_address(smem);
   // The operands of the stage that step i begins, 1 KB a load of a wave; column blocks past the last are that one
   // again, its keys unseen.
   auto load = [&](int i) AW_INLINE {
-    if (cb0 + i * A::CG >= cbs) return;
+    if (i >= steps) return;
     const uint32_t to = lds + (i / A::SB & 1) * A::B;
     for (int k = w; k < A::B / 1024; k += 8) {
       const int group = k / A::ALL;
@@ -479,12 +484,11 @@ __global__ __launch_bounds__(512, 2) void attn_mass_kernel(AttnRowsParams p) {
   };
   auto column = [&](int i) AW_INLINE { return (cb0 + i * A::CG + cg) * 32 + j; };
   auto norm_of = [&](int i) AW_INLINE { return norms[min(column(i), p.cols - 1)]; };
-  const int steps = (cbs - cb0 + A::CG - 1) / A::CG;
   load(0);
   float4 norm = norm_of(0), after = norm_of(1), now;
   wait_loads_and_block<0>();
   load(A::SB);
-  scores(0, s, [](int) {});
+  if (steps > 0) scores(0, s, [](int) {});
   int i = 0;
   // Before a step's exponentials: where the next one begins a stage, its operands are there for every wave, and the
   // stage behind takes the place of what was read last.
@@ -521,7 +525,7 @@ __global__ __launch_bounds__(512, 2) void attn_mass_kernel(AttnRowsParams p) {
   // Steps [i0, i1) are whole: every column sees every key of the wave, and another step follows.
   const int from = (max(0, x0 + 32 * A::KT - 1 - b.cached) * p.rep + 31) / 32;
   const int i0 = min(steps, max(0, from - cg - cb0 + A::CG - 1) / A::CG);
-  const int i1 = max(i0, min(steps - 1, max(0, p.cols / 32 - cg - cb0 + A::CG - 1) / A::CG));
+  const int i1 = max(i0, min(max(0, steps - 1), max(0, p.cols / 32 - cg - cb0 + A::CG - 1) / A::CG));
   masked(i0);
   f32x16_t next[A::KT];
   while (i + 1 < i1) {
@@ -548,8 +552,23 @@ __global__ __launch_bounds__(512, 2) void attn_mass_kernel(AttnRowsParams p) {
   float v = 0.f;
 #pragma unroll
   for (int i = 0; i < A::CG; ++i) v += part[i][threadIdx.x];
+  if (gridDim.y > 1) {
+    p.partial[((size_t)blockIdx.y * gridDim.x + blockIdx.x) * A::KEYS + threadIdx.x] = v;
+    return;
+  }
   float* m = p.mass + (size_t)b.g * p.tail_slots + x;
   *m = x < b.cached ? *m + v : v;
+}
+
+// The parts' sums of the columns into the masses, in order.
+__global__ __launch_bounds__(kArMassBlock) void attn_mass_add(AttnRowsParams p, int parts) {
+  const int kb = blockIdx.x / (unsigned)p.n_kv, g = (int)blockIdx.x - kb * p.n_kv, x = kb * kArMassBlock + threadIdx.x;
+  int have, fresh, pos;
+  if (!ar_sequence(p, 0, have, fresh) || !ar_position(p, pos) || x >= have + fresh) return;
+  float v = 0.f;
+  for (int y = 0; y < parts; ++y) v += p.partial[((size_t)y * gridDim.x + blockIdx.x) * kArMassBlock + threadIdx.x];
+  float* m = p.mass + (size_t)g * p.tail_slots + x;
+  *m = x < have ? *m + v : v;
 }
 
 // Launch ------------------------------------------------------------------------------------------
@@ -682,7 +701,11 @@ static size_t ar_norm_bytes(const AttnRowsParams& p) { return (size_t)p.n * p.n_
 static size_t ar_plane_bytes(const AttnRowsParams& p) {
   return (size_t)cdiv(p.n * (p.n_head / p.n_kv), 32) * 32 * p.n_kv * p.hd * (p.half_io ? 2 : 4);
 }
-size_t attn_mass_work_bytes(const AttnRowsParams& p) { return ar_score_bytes(p) + ar_norm_bytes(p) + ar_plane_bytes(p); }
+// (Parts of the masses: at most kArCus blocks where there are several.)
+constexpr size_t kArPartialBytes = (size_t)kArCus * kArMassBlock * 4;
+size_t attn_mass_work_bytes(const AttnRowsParams& p) {
+  return p.n ? ar_score_bytes(p) + ar_norm_bytes(p) + ar_plane_bytes(p) + kArPartialBytes : 0;
+}
 
 // One segment's blocks, or those of both (few columns each).
 template <int HD, bool HALF, bool MASS>
@@ -713,8 +736,17 @@ static int ar_launch(AttnRowsParams& p, const ArCut& prefix, const ArCut& tail, 
   TRX_LAUNCHED();
   if constexpr (MASS) {
     if (!p.scores) {
-      hipLaunchKernelGGL((attn_mass_kernel<HD, HALF>), dim3(cdiv(ar_most_rows(p), ArMass<HD, HALF>::KEYS) * p.n_kv), dim3(512), 0, s, p);
+      // Few blocks of keys (a prompt's first chunk) share the columns as well, four steps at least each, and a small launch
+      // adds their sums up: 490 positions of 24 heads of 256 alone 64 us, 123 in one part; 538 of 32 heads of 128 over 488
+      // rows 68 and 81.
+      const int blocks = cdiv(ar_most_rows(p), kArMassBlock) * p.n_kv;
+      const int parts = std::max(1, std::min(kArCus / blocks, cdiv(cdiv(p.cols, 32), ArMass<HD, HALF>::CG) / 4));
+      hipLaunchKernelGGL((attn_mass_kernel<HD, HALF>), dim3(blocks, parts), dim3(512), 0, s, p);
       TRX_LAUNCHED();
+      if (parts > 1) {
+        hipLaunchKernelGGL(attn_mass_add, dim3(blocks), dim3(kArMassBlock), 0, s, p, parts);
+        TRX_LAUNCHED();
+      }
     }
   }
   return TRX_OK;
@@ -747,6 +779,7 @@ int launch_attn_rows(const AttnRowsParams& params, hipStream_t s) {
     p.score_ld = ar_score_ld(p);
     p.norms = (float4*)(at + ar_score_bytes(p));
     p.planes = keeps ? nullptr : at + ar_score_bytes(p) + ar_norm_bytes(p);
+    p.partial = (float*)(at + ar_score_bytes(p) + ar_norm_bytes(p) + ar_plane_bytes(p));
   }
   if (p.half_io) {
     if (p.hd == 64) return ar_launch<64, true>(p, prefix, tail, s);
