@@ -264,9 +264,8 @@ int trx_attn_window(const trx_attn_window_shape* shape, int n, int pos, const in
  * both at most 2^30 / n_kv_head, n_head <= 1024, batch * n * n_head <= 2^23 (batch or n 0: nothing is done). out,
  * workspace and the tails overlap no other argument.
  * Scores, maxima and sums are fp32. How keys and columns are cut depends on the batch, and with it the last bits of a
- * draft's outputs; the same call gives the same bits. With TRX_KIND_F16 a prefix under more than 32 columns (batch * n
- * times the heads of a kv head) and a tail under more than 32 (n times the heads) may also round each probability to
- * fp16, by 2^-11 of itself.
+ * draft's outputs before they are rounded; the same call gives the same bits. With TRX_KIND_F16 q, gate and
+ * out are fp16, and nothing else is rounded to it.
  * workspace: trx_attn_shared_geometry's bytes, which hold any call of the shape of up to `batch` drafts, `n` new
  * rows and any prefix, no zeroing needed; calls that share it must not overlap. */
 typedef struct trx_attn_shared_shape {
@@ -300,8 +299,7 @@ int trx_attn_shared(const trx_attn_shared_shape* shape, int batch, int n, int pr
  * the masses of its kv head NaN. slots <= 2^30 / n_kv_head, n_head <= 1024, n * n_head <= 2^23 (n = 0: nothing is done).
  * out, workspace and the cache's arrays overlap no other argument.
  * Masses are sums in fp32 of probabilities in fp32; they do not depend on the order of blocks: the same call gives the
- * same bits. With TRX_KIND_F16 calls of more than 32 columns (n times the heads of a kv head) may round each
- * probability to fp16 in the outputs, by 2^-11 of itself.
+ * same bits. With TRX_KIND_F16 q, gate and out are fp16, and nothing else is rounded to it.
  * workspace: trx_attn_mass_geometry's bytes for n, which hold any call of the shape of up to n positions, no
  * zeroing needed; calls that share it must not overlap.
  *

@@ -98,6 +98,11 @@ struct ArLine {
   using Block = ArBlock;
   using Rows = ArRows<HD>;
   using Column = ArColumn;
+  // fp16 calls of many columns take both planes of the probabilities, as those of few: fp16 outputs are the fp32 result
+  // rounded, however many drafts share the call (2.1e-4 of the result's norm against 64 bits; 2.9e-4 with one plane). The
+  // second one is a third of the products: 64 drafts over 32768 rows 107 us, 95 with one; 1021 positions over 7001 rows 280
+  // and 237.
+  static constexpr bool TWO = true;
 
   // A kv head's blocks stay on the XCDs of its number (blocks go round-robin over them), so that the prefix and a
   // sequence's rows are read into few L2s.
@@ -176,8 +181,9 @@ struct ArLine {
   }
 };
 
-// Many columns (aw_many): 256 of 64 fp16 drafts over a prefix of 32768 rows, 8 kv heads of 128, 50 us, 0.69 PFLOP/s; a chunk of
-// 1024 fp32 positions over 2900 rows 130 us, 0.88 with both planes counted; bound as the window attention's chunks.
+// Many columns (aw_many): 256 of 64 fp16 drafts over a prefix of 32768 rows, 8 kv heads of 128, 62 us, 0.83 PFLOP/s with the
+// probabilities' two planes counted; a chunk of 1024 fp32 positions over 2900 rows 117 us, 0.98 with both planes of all;
+// bound as the window attention's chunks.
 template <int HD, bool HALF, bool MASS, int WQ, int WK, int D>
 __global__ __launch_bounds__(64 * WQ * WK, WQ * WK / 4) void attn_rows_kernel(AttnRowsParams p) {
   aw_many<ArLine<HD, HALF, MASS>, HD, HALF, WQ, WK, D>(p);
@@ -588,19 +594,20 @@ static int ar_most_rows(const AttnRowsParams& p) { return p.state || p.lengths ?
 
 // What a cut of a segment takes by this estimate, in microseconds, with `others` blocks beside it: a block takes a fixed
 // part (its queries, the first rows' latency, the join of its waves, the outputs) and a step for each wk tiles of keys;
-// a full chip makes a step 1.4 times as long. Measured (us; waves of columns and splits of the prefix, splits of the
+// a full chip makes a step 1.4 times as long. fp16 queries, one plane against fp32's two, leave three of four products, a step
+// of wide blocks 0.72 as long. Measured (us; waves of columns and splits of the prefix, splits of the
 // tails), the choice first:
 //   24 drafts over 4001 rows and up to 300 of their own, 32 heads of 128, 8 kv heads: (1, 12; 1) 20; (1, 8; 1) 20,
 //     (1, 4; 1) 25, (1, 16; 2) 27, (4, 32; 1) 35
-//   64 over 32768 and up to 999, fp16: (4, 16; 1) 93; (4, 8; 1) 106, (2, 8; 1) 109, (4, 24; 1) 109, (1, 8; 1) 130
-//   12 of 7 rows over 6001 and up to 200, fp16: (4, 10; 2) 35; (4, 8; 2) 36, (2, 4; 2) 36, (1, 8; 1) 39, (4, 16; 2) 44
+//   64 over 32768 and up to 999, fp16: (4, 16; 1) 107; (4, 12; 1) 109, (2, 8; 1) 109, (4, 8; 1) 123, (1, 8; 1) 133
+//   12 of 7 rows over 6001 and up to 200, fp16: (4, 10; 2) 39; (4, 8; 2) 39, (2, 4; 2) 40, (1, 8; 1) 41, (4, 6; 2) 42
 //   8 over 2047 and up to 130, 24 heads of 256, 4 kv heads: (1, 16; 2) 20; (1, 8; 1) 23, (2, 16; 1) 39
 //   one token with masses over 32700, fp16: 32 splits 38; 24 41, 64 41, 48 43, 16 49
 //   27 with masses over 1900, 24 heads of 256: (1, 8) 27; (1, 10) 27, (1, 6) 30, (1, 4) 35, (2, 16) 41, (1, 12) 42
 static double ar_time(const AttnRowsParams& p, const ArCut& c, int units, int cols, int keys, long long others) {
   const int wk = c.wq == 1 ? 4 : (p.hd == 256 ? 4 : 8) / c.wq;
   const double fixed = c.wq == 1 ? 2 : 11;
-  const double unit = c.wq == 1 ? p.hd / 64.0 : 1.35 * (p.half_io ? 0.56 : 1.0) * (p.hd == 64 ? 0.6 : 1.0);
+  const double unit = c.wq == 1 ? p.hd / 64.0 : 1.35 * (p.half_io ? 0.72 : 1.0) * (p.hd == 64 ? 0.6 : 1.0);
   const double step = c.wq == 2 ? unit * (p.half_io ? 1.75 : p.hd == 256 ? 1.7 : 1.3) : unit;
   const long long blocks = (long long)units * cdiv(cols, 32 * c.wq) * p.n_kv * c.splits + others;
   const int steps = cdiv(cdiv(cdiv(keys, kAwKeys), c.splits), wk);
@@ -622,7 +629,7 @@ static void ar_plan(const AttnRowsParams& p, ArCut& prefix, ArCut& tail) {
   const long long rows = (long long)p.batch * p.n * p.n_head;
   const double part = 8.0 * rows * p.hd / 6e6;       // a part of every column written and read, at 6 TB/s
   // Each segment alone, one launch behind the other (a prefix brings the join with it). Up to 32 columns stay with the
-  // kernel for few: wide blocks would leave most of theirs empty, and round fp16's probabilities for it.
+  // kernel for few: wide blocks would leave most of theirs empty.
   double time = 0, least = 1e300;
   for (int wq : {1, 2, 4}) {
     if (wq > 1 && cols <= 32) break;

@@ -11,7 +11,8 @@
 //   block (false: nothing to do), sight (whether a column sees a key), whole (stages that every column of a wave
 //     sees whole), all_see (one tile); and what a layout may keep of the work: query (a chunk of a wave's, as operands),
 //     scored (a tile's scores, in calls of few columns), total (of a column that one block finishes: its maximum and
-//     sum).
+//     sum);
+//   TWO: whether fp16 calls of many columns take the probabilities' second plane, as all others do.
 #pragma once
 
 #include "trx_internal.h"
@@ -486,7 +487,7 @@ __device__ __forceinline__ uint32_t aw_tr(uint32_t tile, int lane) {
 // 95 against 88 us, and 15 us of 115 with 256 dims, where it had cost spilled registers.
 template <class Layout, int HD, bool HALF, int WQ, int WK, int D>
 __device__ __forceinline__ void aw_many(const typename Layout::Params& p) {
-  using Wave = AwWave<Layout, HD, HALF, !HALF>;
+  using Wave = AwWave<Layout, HD, HALF, !HALF || Layout::TWO>;
   using Lds = AwLds<HD>;
   constexpr int NW = WQ * WK;
   constexpr int SR = WK * kAwKeys;                // keys a stage

@@ -131,6 +131,7 @@ struct AwRing {
   using Block = AwBlock;
   using Rows = AwRows<HD>;
   using Column = AwColumn;
+  static constexpr bool TWO = false;
 
   __device__ __forceinline__ static bool block(const Params& p, int columns, Block& b) {
     int pos;
