@@ -296,7 +296,8 @@ int trx_attn_shared(const trx_attn_shared_shape* shape, int batch, int n, int pr
  * arguments ignored; values out of range there leave everything as it is.
  * kind, head sizes, row strides, alignment and the treatment of infinities and NaN are trx_attn_window's; mass,
  * positions and state are 4-byte aligned. An infinity or NaN in the query or in a key that it sees may also make
- * the masses of its kv head NaN. slots <= 2^30 / n_kv_head, n_head <= 1024, n * n_head <= 2^23 (n = 0: nothing is done).
+ * the masses of its kv head NaN. slots, rounded up to 128, times n_kv_head below 2^30 (trx_kv_evict: slots <= 2^30 /
+ * n_kv_head), n_head <= 1024, n * n_head <= 2^23 (n = 0: nothing is done).
  * out, workspace and the cache's arrays overlap no other argument.
  * Masses are sums in fp32 of probabilities in fp32; they do not depend on the order of blocks: the same call gives the
  * same bits. With TRX_KIND_F16 q, gate and out are fp16, and nothing else is rounded to it.

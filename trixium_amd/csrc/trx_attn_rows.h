@@ -46,8 +46,9 @@ struct AttnRowsParams {
   void* planes;                // the queries as operands, of calls of many columns with masses
 };
 
-// Why a geometry is not taken (null: it is).
+// Why a geometry is not taken (null: it is), and why not for a sequence with masses.
 const char* attn_rows_refuses(const AttnRowsParams& p);
+const char* attn_mass_refuses(const AttnRowsParams& p);
 // Bytes that any call of up to p.batch drafts, p.n new rows and p.prefix prefix rows needs.
 size_t attn_rows_work_bytes(const AttnRowsParams& p);
 // And what a sequence with masses needs besides.

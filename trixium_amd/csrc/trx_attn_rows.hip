@@ -410,6 +410,7 @@ __global__ __launch_bounds__(256) void attn_rows_finish(AttnRowsParams p, int ma
 // them without a pause); without the loads 9 and 12 us less. Scores and exponentials one after the other took 80 and
 // 115, masks in the loop 71 and 96.
 constexpr int kArMassBlock = 128;                   // keys
+constexpr int kArMassThreads = 512;
 template <int HD, bool HALF>
 struct ArMass {
   static constexpr int KT = HD == 256 ? 1 : 2, KW = HD == 256 ? 4 : 2, CG = 8 / KW;
@@ -420,7 +421,7 @@ struct ArMass {
   static constexpr int B = SB * CG * ALL * 1024;               // bytes of a stage
 };
 template <int HD, bool HALF>
-__global__ __launch_bounds__(512, 2) void attn_mass_kernel(AttnRowsParams p) {
+__global__ __launch_bounds__(kArMassThreads, 2) void attn_mass_kernel(AttnRowsParams p) {
   using A = ArMass<HD, HALF>;
   __shared__ __align__(1024) uint8_t smem[2 * A::B];
   __shared__ float part[A::CG][A::KEYS];
@@ -668,7 +669,6 @@ const char* attn_rows_refuses(const AttnRowsParams& p) {
   if (p.n_kv < 1 || p.n_head < 1 || p.n_head % p.n_kv) return "n_head is not a multiple of n_kv_head";
   if (p.n_head > 1024) return "more than 1024 heads";
   if (p.prefix_slots < 0 || p.prefix_slots > 1 << 30 || p.tail_slots < 1 || p.tail_slots > 1 << 30) return "slots outside [1, 2^30]";
-  // (The masses' blocks, of 128 keys, stay below a grid's 2^32 threads.)
   if ((long long)p.tail_slots * p.n_kv > 1 << 30 || (long long)p.prefix_slots * p.n_kv > 1 << 30) return "more than 2^30 slots of all kv heads";
   if (p.prefix < 0 || p.prefix > p.prefix_slots) return "prefix outside [0, prefix_slots]";
   // (Blocks of 256 threads, one a column at most, stay below a grid's 2^32 threads.)
@@ -681,6 +681,14 @@ const char* attn_rows_refuses(const AttnRowsParams& p) {
   if (p.gate && (p.gate_head_stride < p.hd || p.gate_head_stride % o4 || p.gate_stride % o4 ||
                  p.gate_stride < (long long)(p.n_head - 1) * p.gate_head_stride + p.hd))
     return "gate strides";
+  return nullptr;
+}
+
+const char* attn_mass_refuses(const AttnRowsParams& p) {
+  if (const char* why = attn_rows_refuses(p)) return why;
+  // (attn_mass_kernel's blocks, 512 threads for 128 keys of a kv head, stay below a grid's 2^32 threads.)
+  if (((long long)p.tail_slots + kArMassBlock - 1) / kArMassBlock * p.n_kv * kArMassThreads >= 1ll << 32)
+    return "2^30 slots of all kv heads or more";
   return nullptr;
 }
 
@@ -748,7 +756,7 @@ static int ar_launch(AttnRowsParams& p, const ArCut& prefix, const ArCut& tail, 
       // rows 68 and 81.
       const int blocks = cdiv(ar_most_rows(p), kArMassBlock) * p.n_kv;
       const int parts = std::max(1, std::min(kArCus / blocks, cdiv(cdiv(p.cols, 32), ArMass<HD, HALF>::CG) / 4));
-      hipLaunchKernelGGL((attn_mass_kernel<HD, HALF>), dim3(blocks, parts), dim3(512), 0, s, p);
+      hipLaunchKernelGGL((attn_mass_kernel<HD, HALF>), dim3(blocks, parts), dim3(kArMassThreads), 0, s, p);
       TRX_LAUNCHED();
       if (parts > 1) {
         hipLaunchKernelGGL(attn_mass_add, dim3(blocks), dim3(kArMassBlock), 0, s, p, parts);
@@ -766,7 +774,7 @@ static int ar_launch(AttnRowsParams& p, const ArCut& prefix, const ArCut& tail, 
 
 int launch_attn_rows(const AttnRowsParams& params, hipStream_t s) {
   AttnRowsParams p = params;
-  const char* why = attn_rows_refuses(p);
+  const char* why = p.mass ? attn_mass_refuses(p) : attn_rows_refuses(p);
   TRX_CHECK(!why, TRX_E_INVALID, "attention over rows: %s", why);
   if (p.n == 0 || p.batch == 0) return TRX_OK;
   p.rep = p.n_head / p.n_kv;
@@ -888,7 +896,7 @@ TRX_API int trx_attn_mass_geometry(const trx_attn_mass_shape* shape, int n, size
   TRX_CHECK_SHAPE(shape, "trx_attn_mass_geometry");
   TRX_CHECK(workspace_bytes, TRX_E_INVALID, "trx_attn_mass_geometry: null argument");
   AttnRowsParams p = mass_params(shape, n);
-  const char* why = attn_rows_refuses(p);
+  const char* why = attn_mass_refuses(p);
   TRX_CHECK(!why, TRX_E_INVALID, "trx_attn_mass_geometry: %s", why);
   *workspace_bytes = attn_rows_work_bytes(p) + attn_mass_work_bytes(p);
   return TRX_OK;
@@ -900,7 +908,7 @@ TRX_API int trx_attn_mass(const trx_attn_mass_shape* shape, int n, int count, in
   TRX_CHECK_SHAPE(shape, "trx_attn_mass");
   AttnRowsParams p = mass_params(shape, n);
   p.gate = gate;
-  const char* why = attn_rows_refuses(p);
+  const char* why = attn_mass_refuses(p);
   TRX_CHECK(!why, TRX_E_INVALID, "trx_attn_mass: %s", why);
   TRX_CHECK(n <= shape->slots, TRX_E_INVALID, "trx_attn_mass: %d rows, %d slots", n, shape->slots);
   TRX_CHECK(state || (count >= 0 && count <= shape->slots - n), TRX_E_INVALID, "trx_attn_mass: %d rows and %d new ones, %d slots",

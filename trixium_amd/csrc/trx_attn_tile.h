@@ -107,7 +107,7 @@ template <class Params>
 __device__ __forceinline__ int aw_row(const Params& p, int column) {
   return (int)((unsigned long long)(unsigned)column * p.rep_m >> p.rep_s);
 }
-// The first of a split's share of `count` stages (count below 2^26, at most 64 splits).
+// The first of a split's share of `count` stages (count times splits below 2^32).
 __device__ __forceinline__ int aw_share(int count, int split, int splits) {
   return (int)((unsigned)count * (unsigned)split / (unsigned)splits);
 }
