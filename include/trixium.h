@@ -305,8 +305,10 @@ int trx_attn_shared(const trx_attn_shared_shape* shape, int batch, int n, int pr
  * zeroing needed; calls that share it must not overlap.
  *
  * trx_kv_evict: of the `count` rows of every kv head, `keep` stay: those at positions below `sinks` or from
- * pos - recent on (pos: the next row's position) before any other, then those of the largest masses (a NaN is
- * below every number), equal ones by slot. Of what stays, the rows from slot `keep` on take the slots below it of
+ * pos - recent on (pos: the next row's position) before any other, then those of the largest masses (an infinity is
+ * the largest, a NaN below every number), equal ones by slot. Where more than `keep` rows are at such positions, those in
+ * the lowest slots stay, whatever their masses and positions: with sinks + recent <= keep that does not happen to a cache
+ * that holds a position once. Of what stays, the rows from slot `keep` on take the slots below it of
  * rows that go, first to first; K, V, mass and position of a row move together. The cache then holds `keep` rows;
  * nothing else is written. keep >= count: nothing is done. 1 <= keep <= slots, 0 <= count <= slots, sinks >= 0,
  * recent >= 0, pos >= 0. Of the shape the heads, head_dim and slots count.

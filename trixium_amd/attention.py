@@ -252,7 +252,8 @@ class KVMass(_Rows):
 
     def evict(self, keep, sinks=4, recent=0):
         """Keeps `keep` rows of each kv head: the first `sinks` positions and the last `recent` before the others,
-        then the largest masses."""
+        then the largest masses. Of more than `keep` rows at such positions (sinks + recent > keep) those in the lowest
+        slots stay."""
         _int32s(keep=keep, sinks=sinks, recent=recent)
         work = self._workspace("trx_kv_evict_geometry")
         _lib.call("trx_kv_evict", ctypes.byref(self.shape), self.count, self.next, None, keep, sinks, recent, self.kcache.ptr,

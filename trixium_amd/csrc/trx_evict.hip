@@ -1,7 +1,8 @@
-// Eviction from a cache with masses (trx_kv_evict): of the `count` rows of a kv head the `keep` foremost stay, in the
-// order (at a position that is kept, mass falling, slot rising), and the rows that stay past slot keep move into
-// the slots of those that go below it. Nothing else moves, so a token's eviction touches one row, and rows are read
-// at slots from keep on and written at slots below it: no order of blocks matters.
+// Eviction from a cache with masses (trx_kv_evict): of the `count` rows of a kv head the `keep` foremost stay, first
+// those at positions that are kept, slot rising (their masses do not count), then the others, mass falling and slot
+// rising; and the rows that stay past slot keep move into the slots of those that go below it. Nothing else moves, so a
+// token's eviction touches one row, and rows are read at slots from keep on and written at slots below it: no order of
+// blocks matters.
 //
 // Selection: a row's key is 32 bits that order as the rows do and 32 of its slot, so that no two are equal; the
 // keep-th largest is found by its bits, 11, 11 and 10 at a time, most significant first, each from a histogram of the
