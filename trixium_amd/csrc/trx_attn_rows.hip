@@ -9,6 +9,7 @@
 //   many columns the scores are taken again, keys staying where the columns pass.
 // No sum depends on the order of blocks.
 
+#include "trx_attn_plan.h"
 #include "trx_attn_rows.h"
 #include "trx_attn_tile.h"
 
@@ -315,7 +316,6 @@ __device__ __forceinline__ void ar_mass_few(const AttnRowsParams& p, int block, 
 
 // Up to 256 columns: the masses of 64 keys a block, each wave a quarter of the columns, the columns' parts joined by a thread
 // each. A block of columns has left scores of the keys that it sees alone.
-constexpr int kArMassColumns = 256;
 __device__ __forceinline__ void ar_mass_some(const AttnRowsParams& p, int block, float2* norm, float* part) {
   const int kb = block / p.n_kv, g = block - kb * p.n_kv, lane = threadIdx.x & 63, w = threadIdx.x >> 6, x = kb * 64 + lane;
   int have, fresh;
@@ -409,14 +409,13 @@ __global__ __launch_bounds__(256) void attn_rows_finish(AttnRowsParams p, int ma
 // 1021 fp16 ones over 7001 rows 94 us (four matrix instructions take a SIMD 66 ns, so that 28 and 31 us would be all of
 // them without a pause); without the loads 9 and 12 us less. Scores and exponentials one after the other took 80 and
 // 115, masks in the loop 71 and 96.
-constexpr int kArMassBlock = 128;                   // keys
 constexpr int kArMassThreads = 512;
 template <int HD, bool HALF>
 struct ArMass {
   static constexpr int KT = HD == 256 ? 1 : 2, KW = HD == 256 ? 4 : 2, CG = 8 / KW;
   static constexpr int KEYS = 32 * KT * KW;                    // a block's
   static constexpr int NC = HD / 16, ALL = HALF ? NC : 2 * NC;  // KB of 32 columns' operands
-  static_assert(KEYS == kArMassBlock, "the parts' layout");
+  static_assert(KEYS == kArMassBlock && CG == ar_mass_group(HD), "the parts' layout");
   static constexpr int SB = HALF ? 2 : 1;                      // steps of CG column blocks a stage
   static constexpr int B = SB * CG * ALL * 1024;               // bytes of a stage
 };
@@ -580,88 +579,11 @@ __global__ __launch_bounds__(kArMassBlock) void attn_mass_add(AttnRowsParams p, 
 
 // Launch ------------------------------------------------------------------------------------------
 
-constexpr int kArCus = 256;
-constexpr int kArMaxSplits = 64;
-constexpr int kArPartRows = 32768;                  // (column, split) pairs of all kv heads that a split segment takes
-
-// How a segment (the prefix under all columns, or the tails under their own) is cut: columns a block, in waves of 32
-// (1: the kernel for few columns), and splits of the keys.
-struct ArCut {
-  int wq, splits;
-};
-
+static_assert(kArTile == kAwKeys, "the plan's tiles");
 // The rows that a tail has at most after the call.
 static int ar_most_rows(const AttnRowsParams& p) { return p.state || p.lengths ? p.tail_slots : p.length + p.n; }
-
-// What a cut of a segment takes by this estimate, in microseconds, with `others` blocks beside it: a block takes a fixed
-// part (its queries, the first rows' latency, the join of its waves, the outputs) and a step for each wk tiles of keys;
-// a full chip makes a step 1.4 times as long. fp16 queries, one plane against fp32's two, leave three of four products, a step
-// of wide blocks 0.72 as long. Measured (us; waves of columns and splits of the prefix, splits of the
-// tails), the choice first:
-//   24 drafts over 4001 rows and up to 300 of their own, 32 heads of 128, 8 kv heads: (1, 12; 1) 20; (1, 8; 1) 20,
-//     (1, 4; 1) 25, (1, 16; 2) 27, (4, 32; 1) 35
-//   64 over 32768 and up to 999, fp16: (4, 16; 1) 107; (4, 12; 1) 109, (2, 8; 1) 109, (4, 8; 1) 123, (1, 8; 1) 133
-//   12 of 7 rows over 6001 and up to 200, fp16: (4, 10; 2) 39; (4, 8; 2) 39, (2, 4; 2) 40, (1, 8; 1) 41, (4, 6; 2) 42
-//   8 over 2047 and up to 130, 24 heads of 256, 4 kv heads: (1, 16; 2) 20; (1, 8; 1) 23, (2, 16; 1) 39
-//   one token with masses over 32700, fp16: 32 splits 38; 24 41, 64 41, 48 43, 16 49
-//   27 with masses over 1900, 24 heads of 256: (1, 8) 27; (1, 10) 27, (1, 6) 30, (1, 4) 35, (2, 16) 41, (1, 12) 42
-static double ar_time(const AttnRowsParams& p, const ArCut& c, int units, int cols, int keys, long long others) {
-  const int wk = c.wq == 1 ? 4 : (p.hd == 256 ? 4 : 8) / c.wq;
-  const double fixed = c.wq == 1 ? 2 : 11;
-  const double unit = c.wq == 1 ? p.hd / 64.0 : 1.35 * (p.half_io ? 0.72 : 1.0) * (p.hd == 64 ? 0.6 : 1.0);
-  const double step = c.wq == 2 ? unit * (p.half_io ? 1.75 : p.hd == 256 ? 1.7 : 1.3) : unit;
-  const long long blocks = (long long)units * cdiv(cols, 32 * c.wq) * p.n_kv * c.splits + others;
-  const int steps = cdiv(cdiv(cdiv(keys, kAwKeys), c.splits), wk);
-  const double full = (double)blocks / kArCus, rounds = full <= 1 ? 1 : 0.5 * (full + std::ceil(full));
-  return rounds * (fixed + steps * step * (1 + 0.4 * std::min(full, 1.0)));
-}
-
-// f of every cut of a segment into splits that its parts have room for.
-template <class F>
-static void ar_cuts(int wq, int keys, long long rows, F f) {
-  for (int s : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64}) {
-    if (s > 1 && (s > cdiv(keys, kAwKeys) || s * rows > kArPartRows)) return;
-    f(ArCut{wq, s});
-  }
-}
-
-static void ar_plan(const AttnRowsParams& p, ArCut& prefix, ArCut& tail) {
-  const int rep = p.n_head / p.n_kv, cols = p.n * rep, all = p.batch * cols, keys = ar_most_rows(p);
-  const long long rows = (long long)p.batch * p.n * p.n_head;
-  const double part = 8.0 * rows * p.hd / 6e6;       // a part of every column written and read, at 6 TB/s
-  // Each segment alone, one launch behind the other (a prefix brings the join with it). Up to 32 columns stay with the
-  // kernel for few: wide blocks would leave most of theirs empty.
-  double time = 0, least = 1e300;
-  for (int wq : {1, 2, 4}) {
-    if (wq > 1 && cols <= 32) break;
-    ar_cuts(wq, keys, rows, [&](const ArCut& c) {
-      const double t = ar_time(p, c, p.batch, cols, keys, 0) + (c.splits > 1 ? (p.prefix ? 0 : 2) + c.splits * part : 0);
-      if (t < least) least = t, tail = c;
-    });
-  }
-  prefix = {1, 0};
-  if (p.prefix > 0) {
-    time = least + 2;
-    least = 1e300;
-    for (int wq : {1, 2, 4}) {
-      if (wq > 1 && all <= 32) break;
-      ar_cuts(wq, p.prefix, rows, [&](const ArCut& c) {
-        const double t = ar_time(p, c, 1, all, p.prefix, 0) + c.splits * part;
-        if (t < least) least = t, prefix = c;
-      });
-    }
-    time += least;
-    // Both in one launch, of few columns a block.
-    ar_cuts(1, keys, rows, [&](const ArCut& b) {
-      const long long tails = (long long)p.batch * cdiv(cols, 32) * p.n_kv * b.splits;
-      ar_cuts(1, p.prefix, rows, [&](const ArCut& a) {
-        const long long prefixes = (long long)cdiv(all, 32) * p.n_kv * a.splits;
-        const double t = std::max(ar_time(p, a, 1, all, p.prefix, tails), ar_time(p, b, p.batch, cols, keys, prefixes)) +
-                         (a.splits + b.splits) * part;
-        if (t < time) time = t, prefix = a, tail = b;
-      });
-    });
-  }
+static ArCall ar_call(const AttnRowsParams& p) {
+  return {p.half_io, p.batch, p.n, p.n_head, p.n_kv, p.hd, p.prefix, p.tail_slots, ar_most_rows(p)};
 }
 
 const char* attn_rows_refuses(const AttnRowsParams& p) {
@@ -692,23 +614,13 @@ const char* attn_mass_refuses(const AttnRowsParams& p) {
   return nullptr;
 }
 
-static long long ar_score_ld(const AttnRowsParams& p) { return ((long long)p.tail_slots + 31) / 32 * 32; }
-// Scores are kept of up to 32 columns, however long the cache, and of up to 256 in 16 MB. (27 positions of 24 heads of 256 over
-// 1900 rows, 5 MB: 27 us, 36 where they are taken again; of 32 heads of 128 over 4000, 14 MB: 26 and 31; 60 of them, 31 MB: 41
-// and 41.)
-constexpr size_t kArScoreBytes = 16 << 20;
-static bool ar_keeps(const AttnRowsParams& p, const ArCut& tail) {
-  const int cols = p.n * (p.n_head / p.n_kv);
-  return cols <= 32 || (tail.wq == 1 && cols <= kArMassColumns && (size_t)cols * p.n_kv * ar_score_ld(p) * 4 <= kArScoreBytes);
-}
-
 // Parts of the prefix and of the tails: one split of each, or as many as kArPartRows allows.
 static size_t ar_parts_bytes(const AttnRowsParams& p) {
   const long long rows = (long long)p.batch * p.n * p.n_head;
   return (size_t)(2 * std::min(std::max<long long>(rows, kArPartRows), kArMaxSplits * rows)) * (p.hd + 2) * 4;
 }
 static size_t ar_score_bytes(const AttnRowsParams& p) {
-  const size_t column = (size_t)p.n_kv * ar_score_ld(p) * 4, cols = (size_t)p.n * (p.n_head / p.n_kv);
+  const size_t column = (size_t)p.n_kv * ar_score_ld(p.tail_slots) * 4, cols = (size_t)p.n * (p.n_head / p.n_kv);
   return std::max(std::min<size_t>(cols, 32) * column, std::min(cols * column, kArScoreBytes));
 }
 size_t attn_rows_work_bytes(const AttnRowsParams& p) { return ar_parts_bytes(p); }
@@ -751,11 +663,7 @@ static int ar_launch(AttnRowsParams& p, const ArCut& prefix, const ArCut& tail, 
   TRX_LAUNCHED();
   if constexpr (MASS) {
     if (!p.scores) {
-      // Few blocks of keys (a prompt's first chunk) share the columns as well, four steps at least each, and a small launch
-      // adds their sums up: 490 positions of 24 heads of 256 alone 64 us, 123 in one part; 538 of 32 heads of 128 over 488
-      // rows 68 and 81.
-      const int blocks = cdiv(ar_most_rows(p), kArMassBlock) * p.n_kv;
-      const int parts = std::max(1, std::min(kArCus / blocks, cdiv(cdiv(p.cols, 32), ArMass<HD, HALF>::CG) / 4));
+      const int blocks = cdiv(ar_most_rows(p), kArMassBlock) * p.n_kv, parts = ar_mass_parts(ar_call(p));
       hipLaunchKernelGGL((attn_mass_kernel<HD, HALF>), dim3(blocks, parts), dim3(kArMassThreads), 0, s, p);
       TRX_LAUNCHED();
       if (parts > 1) {
@@ -783,15 +691,16 @@ int launch_attn_rows(const AttnRowsParams& params, hipStream_t s) {
   while (1 << (p.rep_s - 32) < p.rep) ++p.rep_s;
   p.rep_m = ((1ull << p.rep_s) + p.rep - 1) / p.rep;
   ArCut prefix, tail;
-  ar_plan(p, prefix, tail);
+  const ArCall call = ar_call(p);
+  ar_plan(call, prefix, tail);
   p.prefix_splits = prefix.splits;
   p.tail_splits = tail.splits;
   p.nsplit = prefix.splits + tail.splits;
   if (p.mass) {
     char* at = (char*)p.work + ar_parts_bytes(p);
-    const bool keeps = ar_keeps(p, tail);
+    const bool keeps = ar_keeps(call, tail);
     p.scores = keeps ? (float*)at : nullptr;
-    p.score_ld = ar_score_ld(p);
+    p.score_ld = ar_score_ld(p.tail_slots);
     p.norms = (float4*)(at + ar_score_bytes(p));
     p.planes = keeps ? nullptr : at + ar_score_bytes(p) + ar_norm_bytes(p);
     p.partial = (float*)(at + ar_score_bytes(p) + ar_norm_bytes(p) + ar_plane_bytes(p));
