@@ -182,9 +182,9 @@ struct ArLine {
   }
 };
 
-// Many columns (aw_many): 256 of 64 fp16 drafts over a prefix of 32768 rows, 8 kv heads of 128, 62 us, 0.83 PFLOP/s with the
-// probabilities' two planes counted; a chunk of 1024 fp32 positions over 2900 rows 117 us, 0.98 with both planes of all;
-// bound as the window attention's chunks.
+// Many columns (aw_many): 256 of 64 fp16 drafts over a prefix of 32768 rows, 8 kv heads of 128, 60 us, 0.86 PFLOP/s with the
+// probabilities' two planes counted; a chunk of 1024 fp32 positions over 2900 rows 121 us, 0.94 with both planes of all, of
+// 1021 fp16 ones over 7001 rows 196, 0.96; bound as the window attention's chunks.
 template <int HD, bool HALF, bool MASS, int WQ, int WK, int D>
 __global__ __launch_bounds__(64 * WQ * WK, WQ * WK / 4) void attn_rows_kernel(AttnRowsParams p) {
   aw_many<ArLine<HD, HALF, MASS>, HD, HALF, WQ, WK, D>(p);
@@ -405,10 +405,10 @@ __global__ __launch_bounds__(256) void attn_rows_finish(AttnRowsParams p, int ma
 // lanes and groups are added at the end. (Columns that stayed while the keys passed would have to add up each key over
 // the lanes.) The queries come as the attention left them, in operands' order, so that a step's bytes come straight
 // into LDS and are read in a row. Eight waves, two a SIMD: the matrix instructions of one run beside the exponentials
-// of both. Of 1024 fp32 positions of 32 heads of 128 over 2900 rows 66 us, 0.87 PFLOP/s with both planes counted, of
-// 1021 fp16 ones over 7001 rows 94 us (four matrix instructions take a SIMD 66 ns, so that 28 and 31 us would be all of
-// them without a pause); without the loads 9 and 12 us less. Scores and exponentials one after the other took 80 and
-// 115, masks in the loop 71 and 96.
+// of both. Of 1024 fp32 positions of 32 heads of 128 over 2900 rows 65 us, 0.88 PFLOP/s with both planes counted, of
+// 1021 fp16 ones over 7001 rows 84 us (four matrix instructions take a SIMD 66 ns, so that 28 and 31 us would be all of
+// them without a pause); without the loads 9 and 12 us less. Scores and exponentials one after the other took 14 and
+// 21 us more, masks in the loop 5 and 2.
 constexpr int kArMassThreads = 512;
 template <int HD, bool HALF>
 struct ArMass {

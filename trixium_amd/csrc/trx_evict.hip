@@ -137,7 +137,8 @@ __global__ __launch_bounds__(kEvThreads) void evict_one_kernel(EvictParams p) {
 
 // R: keys a thread has in LDS (0: none, they are read again). OWN: the block moves its rows itself.
 // Bound by one CU: its loads (32768 rows of 8 kv heads, 2 MB: 9 us with the first histogram beside them), then its vector
-// instructions, each some 0.2 us over the rows: 7 for what follows of the cut, 5 for the bits; 23 in all. Keys in
+// instructions, each some 0.2 us over the rows: 7 for what follows of the cut, 5 for the bits; 23 in all while the masses
+// are in the Infinity Cache, 27 from HBM. Keys in
 // registers took 51 (unrolled steps, each fetched once), lists of rows in place of the bits 20 more.
 template <int R, bool OWN>
 __global__ __launch_bounds__(kEvThreads) void evict_select_kernel(EvictParams p) {
@@ -317,7 +318,7 @@ __global__ __launch_bounds__(kEvThreads) void evict_select_kernel(EvictParams p)
 }
 
 // 16 bytes of K and V a thread, which looks for its rows itself: a chain of some eight loads, 5 us for 3600 rows of each of 8
-// kv heads (15 MB read).
+// kv heads (15 MB read), 17 where they come from HBM.
 __global__ __launch_bounds__(256) void evict_move_kernel(EvictParams p) {
   const int g = blockIdx.x % (unsigned)p.n_kv, seg = p.hd / 8;
   const EvictLists lists(p, g);
