@@ -77,3 +77,36 @@ def test_a_count_on_the_device_far_below_the_slots(slots, counts):
     before = [a.copy() for a in c.arrays()]
     for bad in ((slots + 1, 5), (-1, 5), (slots, -1), (0, 0)):
         assert all(np.array_equal(a.view(np.uint8), b.view(np.uint8)) for a, b in zip(before, c.evict(-1, -1, 30, 0, 0, state=bad))), bad
+
+
+@pytest.mark.gpu
+def test_what_stays_was_there_once():
+    """Of each kv head the positions after an eviction are some of those before it, none twice, at their own rows."""
+    c = Cache(3, 3, 64, 600, seed=34)
+    for g in range(3):
+        c.positions[g, :500] = c.rng.permutation(500)
+    K, positions = c.K.copy(), c.positions.copy()
+    c.K, c.V, c.mass, c.positions = c.evict(500, 500, 300, 5, 40)
+    for g in range(3):
+        stays = c.positions[g, :300]
+        assert np.unique(stays).size == 300 and np.isin(stays, positions[g, :500]).all()
+        at = np.argsort(positions[g, :500])[stays]
+        assert np.array_equal(c.K[g, :300].view(np.uint16), K[g, at].view(np.uint16))
+
+
+@pytest.mark.gpu
+def test_drafts_behind_a_cache_without_rows():
+    """KVMass with nothing in it: an eviction that has nothing to do, no masses, drafts whose prefix is empty."""
+    from trixium_amd.attention import KVMass, SharedPrefix
+    m = KVMass(4, 2, 64, 16)
+    m.evict(5)
+    assert m.count == 0 and m.masses().shape == m.positions().shape == (2, 0) and m.rows()[0].shape == (2, 0, 64)
+    none = np.zeros((2, 0, 64), np.float16)
+    rng = np.random.default_rng(35)
+    q, k, v = rng.standard_normal((3, 1, 4, 64)), rng.standard_normal((3, 1, 2, 64)), rng.standard_normal((3, 1, 2, 64))
+    for d in (m.share(3, 4), SharedPrefix(4, 2, 64, none, none, 3, 4)):
+        # One key: its value, whatever the score, but for the probability's planes (2^-22 of it) and what is rounded of
+        # products, sum and reciprocal (2^-24 each, fewer than eight).
+        want = np.repeat(v.astype(np.float16), 2, axis=2).astype(np.float64)
+        assert (np.abs(d.attend(q, k, v) - want) <= np.abs(want) * 2.0**-20).all()
+        assert np.array_equal(d.rows(-1)[0], k[2].astype(np.float16).transpose(1, 0, 2))
